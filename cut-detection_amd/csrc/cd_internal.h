@@ -182,6 +182,31 @@ int launch_nv12_to_bgr(const uint8_t* y, const uint8_t* uv, int n, int W0, int64
                        uint8_t* dst, int chan_order, hipStream_t s);
 int launch_eval_accumulate(const float* logits, const int64_t* labels, int64_t n, int ncls, int64_t* correct,
                            int64_t* total, double* loss_sum, hipStream_t s);
+// rows of class scores (kernels_rows.hip); strides in elements
+constexpr int kMaxTop = 64;         // alternatives of a row
+constexpr int kMaxTeacher = 256;    // teacher entries of a row
+struct RowsIn {
+    const void* x;
+    int type;                       // CD_T_*
+    int64_t n, stride;
+    int k;
+    float temperature;
+};
+struct TeacherIn {
+    const int64_t* ids;             // [n][entries]
+    const void* scores;             // [n][entries] of `type`
+    int type, entries;
+    const float* weights;           // [n] or NULL
+};
+size_t rows_workspace(int64_t n, int k, int type, int top);
+int launch_log_probs(const RowsIn& in, const int64_t* ids, int top, float* stats, float* logp, float* entropy,
+                     float* top_logp, int64_t* top_ids, void* workspace, hipStream_t s);
+int launch_log_probs_backward(const RowsIn& in, const int64_t* ids, const float* stats, const float* entropy,
+                              const float* g_logp, const float* g_entropy, void* dx, int64_t dx_stride, hipStream_t s);
+int launch_distill(const RowsIn& in, const TeacherIn& te, float* stats, float* loss, void* dx, int64_t dx_stride,
+                   void* workspace, hipStream_t s);
+int launch_distill_backward(const RowsIn& in, const TeacherIn& te, const float* stats, const float* g_loss, void* dx,
+                            int64_t dx_stride, hipStream_t s);
 int launch_synth(uint8_t* dst, int n, int H0, int W0, const uint8_t* classes, uint32_t seed,
                  int64_t first_index, hipStream_t s);
 

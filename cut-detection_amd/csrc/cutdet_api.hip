@@ -508,6 +508,64 @@ struct DeviceGuard {
     ~DeviceGuard() { if (prev >= 0) (void)hipSetDevice(prev); }
 };
 
+// the checks that the calls on rows of class scores share
+int check_rows(const char* name, const cd_handle* h, const RowsIn& in) {
+    if (!h || !in.x) { set_error("%s: null argument", name); return CD_EINVAL; }
+    if (in.type != CD_T_F32 && in.type != CD_T_BF16 && in.type != CD_T_F16) {
+        set_error("%s: score type %d", name, in.type);
+        return CD_EINVAL;
+    }
+    if (in.n < 1 || in.k < 1 || in.k > (1 << 30) || in.n > ((int64_t)1 << 40)) {
+        set_error("%s: %lld rows of %d classes", name, (long long)in.n, in.k);
+        return CD_EINVAL;
+    }
+    if (in.stride < 0 || in.stride > ((int64_t)1 << 40) / in.n * 256) {
+        set_error("%s: row stride %lld", name, (long long)in.stride);
+        return CD_EINVAL;
+    }
+    if (!(in.temperature >= 0x1p-16f && in.temperature <= 0x1p16f)) {
+        set_error("%s: temperature %g outside 2^-16 .. 2^16", name, (double)in.temperature);
+        return CD_EINVAL;
+    }
+    if (reinterpret_cast<uintptr_t>(in.x) % (in.type == CD_T_F32 ? 4 : 2)) {
+        set_error("%s: misaligned scores", name);
+        return CD_EINVAL;
+    }
+    return CD_OK;
+}
+int check_grad(const char* name, const RowsIn& in, const void* grad, int64_t stride) {
+    const int size = in.type == CD_T_F32 ? 4 : 2;
+    if (reinterpret_cast<uintptr_t>(grad) % size || stride < in.k || stride > ((int64_t)1 << 40) / in.n * 256) {
+        set_error("%s: gradient misaligned or its row stride %lld below %d classes", name, (long long)stride, in.k);
+        return CD_EINVAL;
+    }
+    const char *a = static_cast<const char*>(in.x), *b = static_cast<const char*>(grad);
+    const char *a1 = a + ((in.n - 1) * in.stride + in.k) * size, *b1 = b + ((in.n - 1) * stride + in.k) * size;
+    const bool own = a == b && (in.n == 1 || in.stride == stride);
+    if (!own && a < b1 && b < a1) {
+        set_error("%s: gradient overlaps with the scores", name);
+        return CD_EINVAL;
+    }
+    return CD_OK;
+}
+int check_workspace(const char* name, const RowsIn& in, int top, const void* p, size_t bytes) {
+    const size_t need = rows_workspace(in.n, in.k, in.type, top);
+    if (need && (!p || bytes < need || reinterpret_cast<uintptr_t>(p) % 16)) {
+        set_error("%s: workspace of %zu bytes, 16-byte aligned, needed (got %zu)", name, need, p ? bytes : (size_t)0);
+        return CD_ECAP;
+    }
+    return CD_OK;
+}
+int check_teacher(const char* name, const TeacherIn& te) {
+    if (!te.ids || !te.scores || (te.type != CD_T_F32 && te.type != CD_T_BF16 && te.type != CD_T_F16) ||
+        reinterpret_cast<uintptr_t>(te.scores) % (te.type == CD_T_F32 ? 4 : 2) || te.entries < 1 ||
+        te.entries > kMaxTeacher) {
+        set_error("%s: null or misaligned teacher, type %d, or %d entries (1..%d)", name, te.type, te.entries, kMaxTeacher);
+        return CD_EINVAL;
+    }
+    return CD_OK;
+}
+
 }  // namespace
 }  // namespace cd
 
@@ -959,6 +1017,77 @@ int cd_eval_accumulate(cd_handle* h, const float* logits, const int64_t* labels,
     DeviceGuard guard(h->device);
     return launch_eval_accumulate(logits, labels, n, n_classes, correct, total, loss_sum,
                                   static_cast<hipStream_t>(stream));
+}
+
+size_t cd_rows_workspace(int64_t n, int n_classes, int score_type, int top) {
+    if (n < 1 || n_classes < 1 || top < 0 || top > kMaxTop) return 0;
+    return rows_workspace(n, n_classes, score_type, top);
+}
+
+int cd_log_probs(cd_handle* h, const void* scores, int score_type, int64_t n, int n_classes, int64_t row_stride,
+                 float temperature, const int64_t* ids, int top, float* stats, float* logp, float* entropy,
+                 float* top_logp, int64_t* top_ids, void* workspace, size_t workspace_bytes, void* stream) {
+    const RowsIn in = {scores, score_type, n, row_stride, n_classes, temperature};
+    int rc = check_rows("cd_log_probs", h, in);
+    if (rc) return rc;
+    if (!stats || !ids != !logp || (top && (!top_logp || !top_ids))) {
+        set_error("cd_log_probs: null output, or ids without logp");
+        return CD_EINVAL;
+    }
+    if (top < 0 || top > kMaxTop || top > n_classes) {
+        set_error("cd_log_probs: top %d outside 0..min(%d, %d classes)", top, kMaxTop, n_classes);
+        return CD_EINVAL;
+    }
+    if ((rc = check_workspace("cd_log_probs", in, top, workspace, workspace_bytes))) return rc;
+    DeviceGuard guard(h->device);
+    return launch_log_probs(in, ids, top, stats, logp, entropy, top_logp, top_ids, workspace,
+                            static_cast<hipStream_t>(stream));
+}
+
+int cd_log_probs_backward(cd_handle* h, const void* scores, int score_type, int64_t n, int n_classes,
+                          int64_t row_stride, float temperature, const int64_t* ids, const float* stats,
+                          const float* entropy, const float* grad_logp, const float* grad_entropy, void* grad,
+                          int64_t grad_stride, void* stream) {
+    const RowsIn in = {scores, score_type, n, row_stride, n_classes, temperature};
+    int rc = check_rows("cd_log_probs_backward", h, in);
+    if (rc) return rc;
+    if (!stats || !grad || (grad_logp && !ids) || (grad_entropy && !entropy)) {
+        set_error("cd_log_probs_backward: null argument");
+        return CD_EINVAL;
+    }
+    if ((rc = check_grad("cd_log_probs_backward", in, grad, grad_stride))) return rc;
+    DeviceGuard guard(h->device);
+    return launch_log_probs_backward(in, ids, stats, entropy, grad_logp, grad_entropy, grad, grad_stride,
+                                     static_cast<hipStream_t>(stream));
+}
+
+int cd_distill(cd_handle* h, const void* scores, int score_type, int64_t n, int n_classes, int64_t row_stride,
+               float temperature, const int64_t* teacher_ids, const void* teacher_scores, int teacher_type, int entries,
+               const float* weights, float* stats, float* loss, void* grad, int64_t grad_stride, void* workspace,
+               size_t workspace_bytes, void* stream) {
+    const RowsIn in = {scores, score_type, n, row_stride, n_classes, temperature};
+    const TeacherIn te = {teacher_ids, teacher_scores, teacher_type, entries, weights};
+    int rc = check_rows("cd_distill", h, in);
+    if (rc || (rc = check_teacher("cd_distill", te))) return rc;
+    if (!stats || !loss) { set_error("cd_distill: null output"); return CD_EINVAL; }
+    if (grad && (rc = check_grad("cd_distill", in, grad, grad_stride))) return rc;
+    if ((rc = check_workspace("cd_distill", in, 0, workspace, workspace_bytes))) return rc;
+    DeviceGuard guard(h->device);
+    return launch_distill(in, te, stats, loss, grad, grad_stride, workspace, static_cast<hipStream_t>(stream));
+}
+
+int cd_distill_backward(cd_handle* h, const void* scores, int score_type, int64_t n, int n_classes, int64_t row_stride,
+                        float temperature, const int64_t* teacher_ids, const void* teacher_scores, int teacher_type,
+                        int entries, const float* weights, const float* stats, const float* grad_loss, void* grad,
+                        int64_t grad_stride, void* stream) {
+    const RowsIn in = {scores, score_type, n, row_stride, n_classes, temperature};
+    const TeacherIn te = {teacher_ids, teacher_scores, teacher_type, entries, weights};
+    int rc = check_rows("cd_distill_backward", h, in);
+    if (rc || (rc = check_teacher("cd_distill_backward", te))) return rc;
+    if (!stats || !grad_loss || !grad) { set_error("cd_distill_backward: null argument"); return CD_EINVAL; }
+    if ((rc = check_grad("cd_distill_backward", in, grad, grad_stride))) return rc;
+    DeviceGuard guard(h->device);
+    return launch_distill_backward(in, te, stats, grad_loss, grad, grad_stride, static_cast<hipStream_t>(stream));
 }
 
 #ifdef CD_DIAG

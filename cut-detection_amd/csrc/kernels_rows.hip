@@ -1,0 +1,609 @@
+// Operators on rows of class scores x[0..k): log probabilities, entropy and the highest classes of a row, the
+// divergence from a teacher's top classes, and their gradients.
+//
+// With c = log2(e) / T, m = max x and t_i = (x_i - m) c, everything follows from one pass over the row:
+//     S = sum 2^t_i     U = sum 2^t_i t_i
+//     ln p_i = ln2 (t_i - log2 S)        entropy = ln2 (log2 S - U / S)
+// The pass keeps a running maximum per thread; when it rises by d (in units of t), S becomes S 2^-d and U becomes
+// 2^-d (U - d S).  S, U and every statistic are held in 32 bits; the scores stay in the caller's type until they
+// are in registers.
+//
+// Rows without a distribution: -inf scores have probability 0 and add nothing to U (0 log 0 = 0); a row of
+// nothing but -inf has S = 0, log probability -inf everywhere, entropy 0 and gradient 0; a NaN or +inf among the
+// scores makes S, and with it the row's results, NaN.
+#include <algorithm>
+
+#include "cd_internal.h"
+
+namespace cd {
+
+namespace {
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.69314718055994530942f;
+constexpr float kInf = __builtin_inff();
+// t is one fma, x c - fl(m c), while m c is small: what the rounding of m c leaves out is the same for every element of
+// a row and cancels in p, but it has to stay far below 1.  From this magnitude on (and for a row masked with its type's
+// lowest value throughout, where x c would overflow) the difference x - m is formed first.
+constexpr float kPlainLimit = 0x1p20f;
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef u32x4 __attribute__((aligned(2))) u32x4_any;      // 16 bytes at any element's address
+
+template <int TYPE> struct Elem;
+template <> struct Elem<CD_T_F32> {
+    static constexpr int kVec = 4;
+    static constexpr uint32_t kNegInf = 0xff800000u;
+    static __device__ __forceinline__ float load(const char* row, int64_t i) {
+        return reinterpret_cast<const float*>(row)[i];
+    }
+    static __device__ __forceinline__ void store(char* row, int64_t i, float v) { reinterpret_cast<float*>(row)[i] = v; }
+    static __device__ __forceinline__ void unpack(u32x4 w, float* x) {
+        for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(w[i]);
+    }
+    static __device__ __forceinline__ u32x4 pack(const float* x) {
+        u32x4 w;
+        for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(x[i]);
+        return w;
+    }
+};
+template <> struct Elem<CD_T_BF16> {
+    static constexpr int kVec = 8;
+    static constexpr uint32_t kNegInf = 0xff80ff80u;
+    static __device__ __forceinline__ float load(const char* row, int64_t i) {
+        return __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(row)[i] << 16);
+    }
+    static __device__ __forceinline__ void store(char* row, int64_t i, float v) {
+        reinterpret_cast<__bf16*>(row)[i] = (__bf16)v;                    // round to nearest even
+    }
+    static __device__ __forceinline__ void unpack(u32x4 w, float* x) {
+        for (int i = 0; i < 4; ++i) {
+            x[2 * i] = __uint_as_float(w[i] << 16);
+            x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    }
+    static __device__ __forceinline__ u32x4 pack(const float* x) {
+        union { __bf16 h[8]; u32x4 w; } u;
+        for (int i = 0; i < 8; ++i) u.h[i] = (__bf16)x[i];
+        return u.w;
+    }
+};
+template <> struct Elem<CD_T_F16> {
+    static constexpr int kVec = 8;
+    static constexpr uint32_t kNegInf = 0xfc00fc00u;
+    static __device__ __forceinline__ float load(const char* row, int64_t i) {
+        return (float)reinterpret_cast<const _Float16*>(row)[i];
+    }
+    static __device__ __forceinline__ void store(char* row, int64_t i, float v) {
+        reinterpret_cast<_Float16*>(row)[i] = (_Float16)v;                // round to nearest even
+    }
+    static __device__ __forceinline__ void unpack(u32x4 w, float* x) {
+        union { u32x4 w; _Float16 h[8]; } u = {w};
+        for (int i = 0; i < 8; ++i) x[i] = (float)u.h[i];
+    }
+    static __device__ __forceinline__ u32x4 pack(const float* x) {
+        union { _Float16 h[8]; u32x4 w; } u;
+        for (int i = 0; i < 8; ++i) u.h[i] = (_Float16)x[i];
+        return u.w;
+    }
+};
+
+__device__ __forceinline__ float load_any(int type, const void* p, int64_t i) {
+    const char* row = static_cast<const char*>(p);
+    return type == CD_T_F32 ? Elem<CD_T_F32>::load(row, i)
+         : type == CD_T_BF16 ? Elem<CD_T_BF16>::load(row, i) : Elem<CD_T_F16>::load(row, i);
+}
+
+// ---- wave reductions on the DPP network; the result is uniform ---------------------------------------------------
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dpp(float identity, float v) {
+    return __uint_as_float(__builtin_amdgcn_update_dpp(__float_as_uint(identity), __float_as_uint(v), CTRL, ROWS, 0xf, false));
+}
+__device__ __forceinline__ float lane_of(float v, int lane) {
+    return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), lane));
+}
+__device__ __forceinline__ float wave_sum(float v) {      // a NaN in any lane makes the sum NaN
+    v += dpp<0x111, 0xf>(0.f, v);                         // row_shr:1, 2, 4, 8: lane 15 of each row of 16 has its row
+    v += dpp<0x112, 0xf>(0.f, v);
+    v += dpp<0x114, 0xf>(0.f, v);
+    v += dpp<0x118, 0xf>(0.f, v);
+    v += dpp<0x142, 0xa>(0.f, v);                         // row_bcast:15 into rows 1 and 3
+    v += dpp<0x143, 0xc>(0.f, v);                         // row_bcast:31 into rows 2 and 3
+    return lane_of(v, 63);
+}
+__device__ __forceinline__ float wave_max(float v) {      // of numbers (a running maximum is never NaN)
+    v = fmaxf(v, dpp<0x111, 0xf>(-kInf, v));
+    v = fmaxf(v, dpp<0x112, 0xf>(-kInf, v));
+    v = fmaxf(v, dpp<0x114, 0xf>(-kInf, v));
+    v = fmaxf(v, dpp<0x118, 0xf>(-kInf, v));
+    v = fmaxf(v, dpp<0x142, 0xa>(-kInf, v));
+    v = fmaxf(v, dpp<0x143, 0xc>(-kInf, v));
+    return lane_of(v, 63);
+}
+
+// ---- statistics of a row or a part of one ------------------------------------------------------------------------
+struct Stat { float m, s, u; };     // maximum (-inf: nothing but -inf so far), S and U relative to it
+
+__device__ __forceinline__ bool plain(float m, float c) { return fabsf(m * c) < kPlainLimit; }
+
+// t of a score x against a maximum m; the same rounding everywhere, so that S and every p belong together
+struct Ref {
+    float c, mc, m;
+    bool fast;
+    __device__ __forceinline__ Ref(float m_, float c_) : c(c_) {
+        fast = plain(m_, c_);
+        m = m_ == -kInf ? 0.f : m_;
+        mc = fast ? m_ * c_ : 0.f;
+    }
+    __device__ __forceinline__ float operator()(float x) const { return fast ? __builtin_fmaf(x, c, -mc) : (x - m) * c; }
+};
+// t of the maximum `from` against the maximum `to` >= from
+__device__ __forceinline__ float shift(float from, float to, float c) {
+    const bool f = plain(from, c), t = plain(to, c);      // (a plain maximum stands for fl(m c), another for m c itself)
+    return f && t ? from * c - to * c
+         : f ? __builtin_fmaf(-to, c, from * c) : t ? __builtin_fmaf(from, c, -(to * c)) : (from - to) * c;
+}
+__device__ __forceinline__ void rebase(Stat& a, float to, float c) {
+    if (a.m != -kInf && a.m != to) {
+        const float d = shift(a.m, to, c), f = __builtin_amdgcn_exp2f(d);
+        a.u = f * __builtin_fmaf(fmaxf(d, -1e4f), a.s, a.u);
+        a.s *= f;
+    }
+    a.m = to;
+}
+
+template <int N, bool ENT>
+__device__ __forceinline__ void accumulate(const float* x, Stat& a, float c) {
+    float cm = x[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) cm = __builtin_elementwise_maximum(cm, x[i]);
+    if (cm > a.m) rebase(a, cm, c);                       // (not for a NaN: S becomes NaN below)
+    const Ref t_of(a.m, c);
+    if (t_of.fast) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float t = __builtin_fmaf(x[i], c, -t_of.mc), e = __builtin_amdgcn_exp2f(t);
+            a.s += e;
+            if (ENT) a.u = __builtin_fmaf(e, fmaxf(t, -1e4f), a.u);       // the bound: 0 * -inf is 0 here
+        }
+    } else {
+        for (int i = 0; i < N; ++i) {
+            const float t = (x[i] - t_of.m) * c, e = __builtin_amdgcn_exp2f(t);
+            a.s += e;
+            if (ENT) a.u = __builtin_fmaf(e, fmaxf(t, -1e4f), a.u);
+        }
+    }
+}
+
+__device__ __forceinline__ Stat wave_merge(Stat a, float c) {
+    const float m = wave_max(a.m);
+    rebase(a, m, c);
+    a.s = wave_sum(a.s);
+    a.u = wave_sum(a.u);
+    return a;
+}
+
+// ---- order of the classes of a row: 64-bit keys, larger = earlier (NaN, then by score, then by lower index) -----
+__device__ __forceinline__ uint32_t score_key(float x) {
+    if (x != x) return 0xfffffffeu;
+    const uint32_t b = __float_as_uint(x + 0.f);          // -0 counts as +0
+    return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float key_score(uint32_t k) {
+    if (k == 0xfffffffeu) return __builtin_nanf("");
+    return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
+}
+__device__ __forceinline__ uint64_t full_key(float x, uint32_t index) {
+    return (uint64_t)score_key(x) << 32 | (uint32_t)~index;
+}
+__device__ __forceinline__ uint64_t wave_max_key(uint64_t v) {
+    for (int o = 32; o > 0; o >>= 1) {
+        const uint64_t w = __shfl_xor((unsigned long long)v, o);
+        v = w > v ? w : v;
+    }
+    return v;
+}
+
+struct LogProbsArgs {
+    const char* x;
+    int64_t n, row_bytes;
+    int k, top;
+    float c, t;
+    const int64_t* ids;
+    float *stats, *logp, *entropy, *top_logp;
+    int64_t* top_ids;
+};
+
+__device__ __forceinline__ float entropy_of(const Stat& a) {
+    if (a.s == 0.f) return 0.f;
+    const float h = kLn2 * (__builtin_amdgcn_logf(a.s) - a.u / a.s);
+    return h < 0.f ? 0.f : h;
+}
+// ln p of a score; -inf in a row without a distribution
+__device__ __forceinline__ float logp_of(float x, const Stat& a, float c, float temperature) {
+    if (a.s == 0.f) return -kInf;
+    const float t = Ref(a.m, c)(x);
+    if (t < -1e30f && a.s == a.s) return (x - a.m) / temperature;       // in base 2 it could overflow; log S does not count
+    const float lp = kLn2 * (t - __builtin_amdgcn_logf(a.s));
+    return lp > 0.f ? 0.f : lp;
+}
+
+template <int TYPE>
+__device__ __forceinline__ void write_row(const LogProbsArgs& A, int64_t row, const char* x, const Stat& a) {
+    A.stats[2 * row] = a.m;
+    A.stats[2 * row + 1] = a.s;
+    if (A.entropy) A.entropy[row] = entropy_of(a);
+    if (A.logp) {
+        const int64_t id = A.ids[row];
+        A.logp[row] = id >= 0 && id < A.k ? logp_of(Elem<TYPE>::load(x, id), a, A.c, A.t) : 0.f;
+    }
+}
+__device__ __forceinline__ void write_top(const LogProbsArgs& A, int64_t row, int rank, uint64_t key, const Stat& a) {
+    A.top_ids[row * A.top + rank] = (uint32_t)~(uint32_t)key;
+    A.top_logp[row * A.top + rank] = logp_of(key_score((uint32_t)(key >> 32)), a, A.c, A.t);
+}
+
+// ================================================================================== one workgroup per row
+template <int THREADS> struct BlockShared {
+    static constexpr int kWaves = THREADS / 64;
+    float m[kWaves], s[kWaves], u[kWaves];
+    uint64_t key[kWaves];
+};
+
+template <int TYPE, int THREADS, bool ENT>
+__device__ __forceinline__ Stat block_stat(const char* x, int k, float c, BlockShared<THREADS>& sh) {
+    using E = Elem<TYPE>;
+    constexpr int U = 4, VE = E::kVec;
+    const int nv = k / VE, tid = threadIdx.x;
+    Stat a = {-kInf, 0.f, 0.f};
+    for (int v0 = 0; v0 < nv; v0 += U * THREADS) {
+        float xs[U * VE];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int v = v0 + u * THREADS + tid;
+            u32x4 w = {E::kNegInf, E::kNegInf, E::kNegInf, E::kNegInf};
+            if (v < nv) w = reinterpret_cast<const u32x4_any*>(x)[v];
+            E::unpack(w, xs + u * VE);
+        }
+        accumulate<U * VE, ENT>(xs, a, c);
+    }
+    if (nv * VE + tid < k) {
+        const float xt = E::load(x, nv * VE + tid);
+        accumulate<1, ENT>(&xt, a, c);
+    }
+    a = wave_merge(a, c);
+    const int wave = tid >> 6, lane = tid & 63;
+    if (lane == 0) { sh.m[wave] = a.m; sh.s[wave] = a.s; sh.u[wave] = a.u; }
+    __syncthreads();
+    a.m = lane < THREADS / 64 ? sh.m[lane] : -kInf;
+    a.s = lane < THREADS / 64 ? sh.s[lane] : 0.f;
+    a.u = lane < THREADS / 64 ? sh.u[lane] : 0.f;
+    return wave_merge(a, c);
+}
+
+template <int TYPE, int THREADS, bool ENT>
+__global__ __launch_bounds__(THREADS) void log_probs_block_kernel(LogProbsArgs A) {
+    __shared__ BlockShared<THREADS> sh;
+    const int tid = threadIdx.x;
+    for (int64_t row = blockIdx.x; row < A.n; row += gridDim.x) {
+        const char* x = A.x + row * A.row_bytes;
+        const Stat a = block_stat<TYPE, THREADS, ENT>(x, A.k, A.c, sh);
+        if (tid == 0) write_row<TYPE>(A, row, x, a);
+        uint64_t last = ~0ull;
+        for (int r = 0; r < A.top; ++r) {                 // the largest key below the last one found
+            uint64_t best = 0;
+            for (int i = tid; i < A.k; i += THREADS) {
+                const uint64_t key = full_key(Elem<TYPE>::load(x, i), i);
+                if (key < last && key > best) best = key;
+            }
+            best = wave_max_key(best);
+            if ((tid & 63) == 0) sh.key[tid >> 6] = best;
+            __syncthreads();
+            for (int w = 0; w < THREADS / 64; ++w) best = sh.key[w] > best ? sh.key[w] : best;
+            if (tid == 0) write_top(A, row, r, best, a);
+            last = best;
+            __syncthreads();
+        }
+        __syncthreads();
+    }
+}
+
+// ---- gradients ---------------------------------------------------------------------------------------------------
+// d(g_l ln p_id + g_h entropy) / dx_i = [g_l (i == id) - p_i (g_l + g_h (ln p_i + entropy))] / T
+struct LogProbsGradArgs {
+    const char* x;
+    char* dx;
+    int64_t n, row_bytes, dx_row_bytes;
+    int k;
+    float c, inv_t;
+    const int64_t* ids;
+    const float *stats, *entropy, *g_logp, *g_entropy;
+};
+struct GradRow { float a, b, hit; int id; };    // dx_i = 2^t_i (a + b t_i), plus hit at class id
+__device__ __forceinline__ GradRow grad_row(const LogProbsGradArgs& A, int64_t row, float s) {
+    const int64_t id = A.ids ? A.ids[row] : -1;
+    const bool labelled = id >= 0 && id < A.k;
+    const float gl = labelled && A.g_logp ? A.g_logp[row] : 0.f, gh = A.g_entropy ? A.g_entropy[row] : 0.f;
+    GradRow g = {0.f, 0.f, 0.f, -1};
+    if (s == 0.f) return g;
+    const float inv = A.inv_t / s;
+    g.b = -gh * kLn2 * inv;
+    g.a = -(gl + gh * ((A.g_entropy ? A.entropy[row] : 0.f) - kLn2 * __builtin_amdgcn_logf(s))) * inv;
+    g.hit = gl * A.inv_t;
+    g.id = labelled ? (int)id : -1;
+    return g;
+}
+__device__ __forceinline__ float grad_of(float t, const GradRow& g) {
+    return __builtin_amdgcn_exp2f(t) * __builtin_fmaf(g.b, fmaxf(t, -1e4f), g.a);
+}
+
+template <int TYPE, int THREADS>
+__global__ __launch_bounds__(THREADS) void log_probs_grad_kernel(LogProbsGradArgs A) {
+    using E = Elem<TYPE>;
+    for (int64_t row = blockIdx.x; row < A.n; row += gridDim.x) {
+        const char* x = A.x + row * A.row_bytes;
+        char* dx = A.dx + row * A.dx_row_bytes;
+        const float m = A.stats[2 * row], s = A.stats[2 * row + 1];
+        const GradRow g = grad_row(A, row, s);
+        const Ref t_of(m, A.c);
+        const int nv = A.k / E::kVec;
+        for (int v = blockIdx.y * THREADS + threadIdx.x; v < nv; v += gridDim.y * THREADS) {
+            float xs[E::kVec], d[E::kVec];
+            E::unpack(reinterpret_cast<const u32x4_any*>(x)[v], xs);
+#pragma unroll
+            for (int i = 0; i < E::kVec; ++i) d[i] = grad_of(t_of(xs[i]), g);
+            if (g.id >= 0 && g.id / E::kVec == v)
+                for (int i = 0; i < E::kVec; ++i) if (g.id % E::kVec == i) d[i] += g.hit;
+            reinterpret_cast<u32x4_any*>(dx)[v] = E::pack(d);
+        }
+        const int i = nv * E::kVec + threadIdx.x;
+        if (blockIdx.y == 0 && i < A.k) E::store(dx, i, grad_of(t_of(E::load(x, i)), g) + (i == g.id ? g.hit : 0.f));
+    }
+}
+
+// ================================================================================== distillation
+// q = softmax(teacher / T) over the used entries;  loss = w T^2 sum_j q_j (ln q_j - ln p_id_j)
+// dx_i = w T (p_i - sum of q_j with id_j = i)
+struct DistillArgs {
+    const char* x;
+    char* dx;                       // NULL: the loss alone
+    int64_t n, row_bytes, dx_row_bytes;
+    int k, entries, teacher_type;
+    float c, t;
+    const int64_t* ids;
+    const void* teacher;
+    const float *weights;
+    float *stats, *loss;
+};
+constexpr int kTeacherPerLane = kMaxTeacher / 64;
+
+struct Teacher {                    // the entries of one row, spread over a wave: entry lane + 64 e
+    int id[kTeacherPerLane];        // -1: unused
+    float lq[kTeacherPerLane];      // log2 q
+    float q[kTeacherPerLane];       // its share; after `share` of the first entry of a class the sum over its entries
+    float x[kTeacherPerLane];       // the student's score
+    float total;                    // sum of 2^(..) before normalising: 0 where no entry counts
+};
+template <int TYPE>
+__device__ __forceinline__ Teacher load_teacher(const DistillArgs& A, int64_t row, const char* x) {
+    Teacher r;
+    const int lane = threadIdx.x & 63;
+    float m = -kInf;
+#pragma unroll
+    for (int e = 0; e < kTeacherPerLane; ++e) {
+        const int j = lane + 64 * e;
+        int64_t id = -1;
+        float v = -kInf;
+        if (j < A.entries) id = A.ids[row * A.entries + j];
+        const bool used = id >= 0 && id < A.k;
+        if (used) v = load_any(A.teacher_type, A.teacher, row * A.entries + j);
+        r.id[e] = used ? (int)id : -1;
+        r.lq[e] = v;
+        r.x[e] = used ? Elem<TYPE>::load(x, id) : 0.f;
+        m = fmaxf(m, v);
+    }
+    m = wave_max(m);
+    const Ref t_of(m, A.c);
+    float total = 0.f;
+#pragma unroll
+    for (int e = 0; e < kTeacherPerLane; ++e) {
+        r.lq[e] = t_of(r.lq[e]);
+        r.q[e] = r.id[e] >= 0 ? __builtin_amdgcn_exp2f(r.lq[e]) : 0.f;
+        total += r.q[e];
+    }
+    r.total = wave_sum(total);
+    const float l = __builtin_amdgcn_logf(r.total), inv = 1.f / r.total;
+#pragma unroll
+    for (int e = 0; e < kTeacherPerLane; ++e) { r.lq[e] -= l; r.q[e] *= inv; }
+    return r;
+}
+// the row's loss, uniform over the wave
+__device__ __forceinline__ float teacher_loss(const Teacher& r, const Stat& a, const DistillArgs& A, float w) {
+    float sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < kTeacherPerLane; ++e)
+        if (r.id[e] >= 0 && r.q[e] != 0.f)
+            sum = __builtin_fmaf(r.q[e], kLn2 * r.lq[e] - logp_of(r.x[e], a, A.c, A.t), sum);
+    return w * (A.t * A.t) * wave_sum(sum);
+}
+// gradient at the teacher's classes: of a class named twice the first entry has the sum, the others none
+template <int TYPE>
+__device__ __forceinline__ void fix_gradient(const Teacher& r, const Stat& a, const DistillArgs& A, float w, char* dx) {
+    const Ref t_of(a.m, A.c);
+    const float inv = 1.f / a.s;
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int e = 0; e < kTeacherPerLane; ++e) {
+        float sum = 0.f;
+        bool first = r.id[e] >= 0;
+#pragma unroll
+        for (int f = 0; f < kTeacherPerLane; ++f)
+            for (int l = 0; l < min(64, A.entries - 64 * f); ++l) {
+                const int id = __builtin_amdgcn_readlane(r.id[f], l);
+                const float q = lane_of(r.q[f], l);
+                if (id == r.id[e]) {
+                    sum += q;
+                    if (64 * f + l < 64 * e + lane) first = false;
+                }
+            }
+        if (first) Elem<TYPE>::store(dx, r.id[e], w * A.t * (__builtin_amdgcn_exp2f(t_of(r.x[e])) * inv - sum));
+    }
+}
+
+template <int TYPE, int THREADS>
+__global__ __launch_bounds__(THREADS) void distill_block_kernel(DistillArgs A) {
+    using E = Elem<TYPE>;
+    __shared__ BlockShared<THREADS> sh;
+    const int tid = threadIdx.x;
+    for (int64_t row = blockIdx.x; row < A.n; row += gridDim.x) {
+        const char* x = A.x + row * A.row_bytes;
+        char* dx = A.dx + row * A.dx_row_bytes;
+        const float w = A.weights ? A.weights[row] : 1.f;
+        Stat a = {-kInf, 0.f, 0.f};
+        Teacher te;
+        te.total = 0.f;
+        if (w != 0.f) {
+            te = load_teacher<TYPE>(A, row, x);           // (every wave: the total decides for all of them)
+            a = block_stat<TYPE, THREADS, false>(x, A.k, A.c, sh);
+        }
+        const bool on = w != 0.f && te.total != 0.f;
+        if (tid < 64) {
+            const float loss = on ? teacher_loss(te, a, A, w) : 0.f;
+            if (tid == 0) {
+                A.loss[row] = loss;
+                A.stats[2 * row] = a.m;
+                A.stats[2 * row + 1] = a.s;
+            }
+        }
+        if (A.dx) {
+            const Ref t_of(a.m, A.c);
+            const bool live = on && a.s != 0.f;
+            const float f = live ? w * A.t / a.s : 0.f;
+            const int nv = A.k / E::kVec;
+            for (int v = tid; v < nv; v += THREADS) {
+                float d[E::kVec] = {};
+                if (live) {
+                    E::unpack(reinterpret_cast<const u32x4_any*>(x)[v], d);
+#pragma unroll
+                    for (int i = 0; i < E::kVec; ++i) d[i] = f * __builtin_amdgcn_exp2f(t_of(d[i]));
+                }
+                reinterpret_cast<u32x4_any*>(dx)[v] = E::pack(d);
+            }
+            const int i = nv * E::kVec + tid;
+            if (i < A.k) E::store(dx, i, live ? f * __builtin_amdgcn_exp2f(t_of(E::load(x, i))) : 0.f);
+            __syncthreads();
+            if (live && tid < 64) fix_gradient<TYPE>(te, a, A, w, dx);
+        }
+        __syncthreads();
+    }
+}
+
+// the gradient alone, for a loss gradient g per row, from the statistics of the forward call
+struct DistillGradArgs {
+    DistillArgs d;
+    const float* g_loss;
+};
+template <int TYPE, int THREADS>
+__global__ __launch_bounds__(THREADS) void distill_grad_kernel(DistillGradArgs G) {
+    using E = Elem<TYPE>;
+    const DistillArgs& A = G.d;
+    const int tid = threadIdx.x;
+    for (int64_t row = blockIdx.x; row < A.n; row += gridDim.x) {
+        const char* x = A.x + row * A.row_bytes;
+        char* dx = A.dx + row * A.dx_row_bytes;
+        const float w = (A.weights ? A.weights[row] : 1.f);
+        const float wg = w == 0.f ? 0.f : w * G.g_loss[row];
+        const Stat a = {A.stats[2 * row], A.stats[2 * row + 1], 0.f};
+        Teacher te;
+        te.total = 0.f;
+        if (wg != 0.f) te = load_teacher<TYPE>(A, row, x);
+        __syncthreads();                                  // dx may be x: the teacher's classes are read before any write
+        const bool live = wg != 0.f && te.total != 0.f && a.s != 0.f;
+        const Ref t_of(a.m, A.c);
+        const float f = live ? wg * A.t / a.s : 0.f;
+        const int nv = A.k / E::kVec;
+        for (int v = tid; v < nv; v += THREADS) {
+            float d[E::kVec] = {};
+            if (live) {
+                E::unpack(reinterpret_cast<const u32x4_any*>(x)[v], d);
+#pragma unroll
+                for (int i = 0; i < E::kVec; ++i) d[i] = f * __builtin_amdgcn_exp2f(t_of(d[i]));
+            }
+            reinterpret_cast<u32x4_any*>(dx)[v] = E::pack(d);
+        }
+        const int i = nv * E::kVec + tid;
+        if (i < A.k) E::store(dx, i, live ? f * __builtin_amdgcn_exp2f(t_of(E::load(x, i))) : 0.f);
+        __syncthreads();
+        if (live && tid < 64) fix_gradient<TYPE>(te, a, A, wg, dx);
+        __syncthreads();
+    }
+}
+
+constexpr int64_t kMaxGrid = 1 << 20;       // workgroups of a launch; further rows are taken by a loop
+unsigned row_grid(int64_t n) { return (unsigned)std::min(n, kMaxGrid); }
+
+#define CD_BY_TYPE(type, CALL)                       \
+    do {                                             \
+        if ((type) == CD_T_F32) { CALL(CD_T_F32); }  \
+        else if ((type) == CD_T_BF16) { CALL(CD_T_BF16); } \
+        else { CALL(CD_T_F16); }                     \
+    } while (0)
+
+}  // namespace
+
+size_t rows_workspace(int64_t n, int k, int type, int top) { return 0; }
+
+int launch_log_probs(const RowsIn& in, const int64_t* ids, int top, float* stats, float* logp, float* entropy,
+                     float* top_logp, int64_t* top_ids, void* workspace, hipStream_t s) {
+    const LogProbsArgs A = {static_cast<const char*>(in.x), in.n, in.stride * (in.type == CD_T_F32 ? 4 : 2), in.k, top,
+                            kLog2e / in.temperature, in.temperature, ids, stats, logp, entropy, top_logp, top_ids};
+#define CALL(TY)                                                                                                    \
+    if (entropy) log_probs_block_kernel<TY, 256, true><<<row_grid(in.n), 256, 0, s>>>(A);                           \
+    else log_probs_block_kernel<TY, 256, false><<<row_grid(in.n), 256, 0, s>>>(A)
+    CD_BY_TYPE(in.type, CALL);
+#undef CALL
+    CD_HIP(hipGetLastError());
+    return CD_OK;
+}
+
+int launch_log_probs_backward(const RowsIn& in, const int64_t* ids, const float* stats, const float* entropy,
+                              const float* g_logp, const float* g_entropy, void* dx, int64_t dx_stride, hipStream_t s) {
+    const int size = in.type == CD_T_F32 ? 4 : 2;
+    const LogProbsGradArgs A = {static_cast<const char*>(in.x), static_cast<char*>(dx), in.n, in.stride * size,
+                                dx_stride * size, in.k, kLog2e / in.temperature, 1.f / in.temperature, ids, stats,
+                                entropy, g_logp, g_entropy};
+#define CALL(TY) log_probs_grad_kernel<TY, 256><<<row_grid(in.n), 256, 0, s>>>(A)
+    CD_BY_TYPE(in.type, CALL);
+#undef CALL
+    CD_HIP(hipGetLastError());
+    return CD_OK;
+}
+
+static DistillArgs distill_args(const RowsIn& in, const TeacherIn& te, float* stats, float* loss, void* dx,
+                                int64_t dx_stride) {
+    const int size = in.type == CD_T_F32 ? 4 : 2;
+    return {static_cast<const char*>(in.x), static_cast<char*>(dx), in.n, in.stride * size, dx_stride * size, in.k,
+            te.entries, te.type, kLog2e / in.temperature, in.temperature, te.ids, te.scores, te.weights, stats, loss};
+}
+
+int launch_distill(const RowsIn& in, const TeacherIn& te, float* stats, float* loss, void* dx, int64_t dx_stride,
+                   void* workspace, hipStream_t s) {
+    const DistillArgs A = distill_args(in, te, stats, loss, dx, dx_stride);
+#define CALL(TY) distill_block_kernel<TY, 256><<<row_grid(in.n), 256, 0, s>>>(A)
+    CD_BY_TYPE(in.type, CALL);
+#undef CALL
+    CD_HIP(hipGetLastError());
+    return CD_OK;
+}
+
+int launch_distill_backward(const RowsIn& in, const TeacherIn& te, const float* stats, const float* g_loss, void* dx,
+                            int64_t dx_stride, hipStream_t s) {
+    const DistillGradArgs G = {distill_args(in, te, const_cast<float*>(stats), nullptr, dx, dx_stride), g_loss};
+#define CALL(TY) distill_grad_kernel<TY, 256><<<row_grid(in.n), 256, 0, s>>>(G)
+    CD_BY_TYPE(in.type, CALL);
+#undef CALL
+    CD_HIP(hipGetLastError());
+    return CD_OK;
+}
+
+}  // namespace cd

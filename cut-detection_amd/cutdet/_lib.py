@@ -22,6 +22,7 @@ CD_BF16 = 1
 CD_BF16_SPLIT = 2
 DTYPES = {"f32": CD_F32, "bf16": CD_BF16, "bf16_split": CD_BF16_SPLIT}
 CD_BGR, CD_RGB = 0, 1
+CD_T_F32, CD_T_BF16, CD_T_F16 = 0, 1, 2
 OPTIONS = {"range_by_stage": 0, "fuse_blocks12": 1, "range_one_stream": 2, "split_two_waves": 3, "resize_rows": 4, "f32_block1_fp32_mfma": 5}
 STAGES = ("preprocess", "conv1", "conv2", "conv3_head", "rle")
 
@@ -29,6 +30,8 @@ _h = C.c_void_p
 _p = C.c_void_p
 _i = C.c_int
 _l = C.c_int64
+_f = C.c_float
+_z = C.c_size_t
 
 SIGNATURES = {
     "cd_version": (C.c_int, []),
@@ -46,6 +49,11 @@ SIGNATURES = {
     "cd_forward_u8_static": (C.c_int, [_h, _p, _i, _i, _i, _l, _l, _i, _i, _i, _p, _p, _p, _p]),
     "cd_max_argmax": (C.c_int, [_h, _p, _l, _i, _p, _p, _p]),
     "cd_eval_accumulate": (C.c_int, [_h, _p, _p, _l, _i, _p, _p, _p, _p]),
+    "cd_rows_workspace": (C.c_size_t, [_l, _i, _i, _i]),
+    "cd_log_probs": (C.c_int, [_h, _p, _i, _l, _i, _l, _f, _p, _i, _p, _p, _p, _p, _p, _p, _z, _p]),
+    "cd_log_probs_backward": (C.c_int, [_h, _p, _i, _l, _i, _l, _f, _p, _p, _p, _p, _p, _p, _l, _p]),
+    "cd_distill": (C.c_int, [_h, _p, _i, _l, _i, _l, _f, _p, _p, _i, _i, _p, _p, _p, _p, _l, _p, _z, _p]),
+    "cd_distill_backward": (C.c_int, [_h, _p, _i, _l, _i, _l, _f, _p, _p, _i, _i, _p, _p, _p, _p, _l, _p]),
     "cd_rle": (C.c_int, [_h, _p, _p, _l, _l, _p, _p, _p, _p, _p, _p, _l, _p, _p]),
     "cd_synth_frames": (C.c_int, [_h, _p, _i, _i, _i, _p, C.c_uint32, _l, _p]),
     "cd_timing_enable": (C.c_int, [_h, _i]),

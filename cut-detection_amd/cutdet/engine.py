@@ -34,6 +34,9 @@ def _ptr(t):
     return C.c_void_p(t.data_ptr()) if t is not None else C.c_void_p(0)
 
 
+SCORE_TYPES = {torch.float32: _lib.CD_T_F32, torch.bfloat16: _lib.CD_T_BF16, torch.float16: _lib.CD_T_F16}
+
+
 class Engine:
     """One classifier instance on one GPU."""
 
@@ -249,6 +252,156 @@ class Engine:
         if logits.shape[0]:
             check(lib.cd_eval_accumulate(self._h, _ptr(logits), _ptr(labels), logits.shape[0], k, _ptr(correct),
                                          _ptr(total), _ptr(loss_sum), self._stream()))
+
+    # -- rows of class scores (cd_log_probs and the calls after it in cutdet.h)
+    def _score_rows(self, scores):
+        """Rows of scores f32/bf16/f16 [n, k] on the engine's GPU, as they are where a row's elements are
+        consecutive (any row stride, 0 too), else copied."""
+        if not torch.is_tensor(scores) or scores.device != self.device:
+            raise RuntimeError(f"scores must be a tensor on {self.device} (got {getattr(scores, 'device', type(scores))})")
+        if scores.dtype not in SCORE_TYPES:
+            raise TypeError(f"scores must be float32, bfloat16 or float16, got {scores.dtype}")
+        if scores.dim() != 2 or scores.shape[1] < 1:
+            raise ValueError("scores must be [n, k]")
+        return scores if scores.shape[1] == 1 or scores.stride(1) == 1 else scores.contiguous()
+
+    def _per_row(self, t, name, dtype, n, *more):
+        """None, or a tensor [n, *more] of `dtype` on the engine's GPU, made contiguous."""
+        if t is None:
+            return None
+        self._check_dev(t, name, dtype)
+        if tuple(t.shape) != (n, *more):
+            raise ValueError(f"{name} must have shape {(n, *more)}, got {tuple(t.shape)}")
+        return t.contiguous()
+
+    def _grad_rows(self, out, scores):
+        """The tensor to write the scores' gradient to."""
+        if out is None:
+            return torch.empty(scores.shape, dtype=scores.dtype, device=self.device)
+        self._check_dev(out, "out", scores.dtype)
+        n, k = scores.shape
+        if tuple(out.shape) != (n, k) or (k > 1 and out.stride(1) != 1) or (n > 1 and out.stride(0) < k):
+            raise ValueError(f"out must be {scores.dtype} {(n, k)} with consecutive elements in a row and rows apart")
+        return out
+
+    @staticmethod
+    def _row_stride(t):
+        return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+    def _workspace(self, scores, top):
+        n, k = scores.shape
+        size = lib.cd_rows_workspace(n, k, SCORE_TYPES[scores.dtype], top)
+        return torch.empty((size,), dtype=torch.uint8, device=self.device) if size else None, size
+
+    def log_probs(self, scores, ids=None, top=0, temperature=1.0, entropy=True):
+        """Of every row of scores (f32, bf16 or f16 [n, k]; any row stride), with p = softmax(scores / temperature):
+        `logp` [n], the log probability of class ids[row] (int64 [n]; 0 where the id is outside 0..k-1);
+        `entropy` [n]; `top_logp`, `top_ids` [n, top], the classes with the highest scores (at most 64, equal scores
+        in the order of their index); `stats` [n, 2] for log_probs_backward.  A dict of float32 (ids: int64)
+        tensors, without what was not asked for.  See cd_log_probs for -inf, NaN and rows without a distribution."""
+        scores = self._score_rows(scores)
+        n, k = scores.shape
+        top = int(top)
+        if not 0 <= top <= min(64, k):
+            raise ValueError(f"top must be in 0..{min(64, k)}, got {top}")
+        ids = self._per_row(ids, "ids", torch.int64, n)
+        f32 = dict(dtype=torch.float32, device=self.device)
+        out = {"stats": torch.empty((n, 2), **f32)}
+        if ids is not None:
+            out["logp"] = torch.empty((n,), **f32)
+        if entropy:
+            out["entropy"] = torch.empty((n,), **f32)
+        if top:
+            out["top_logp"] = torch.empty((n, top), **f32)
+            out["top_ids"] = torch.empty((n, top), dtype=torch.int64, device=self.device)
+        if n:
+            ws, size = self._workspace(scores, top)
+            check(lib.cd_log_probs(self._h, _ptr(scores), SCORE_TYPES[scores.dtype], n, k, self._row_stride(scores),
+                                   float(temperature), _ptr(ids), top, _ptr(out["stats"]), _ptr(out.get("logp")),
+                                   _ptr(out.get("entropy")), _ptr(out.get("top_logp")), _ptr(out.get("top_ids")),
+                                   _ptr(ws), size, self._stream()))
+        return out
+
+    def log_probs_backward(self, scores, ids, stats, entropy, grad_logp=None, grad_entropy=None, temperature=1.0,
+                           out=None):
+        """Gradient of sum(grad_logp * logp + grad_entropy * entropy) with respect to the scores, in their type.
+        `stats` and `entropy` are those of log_probs on the same scores; `ids` is needed with `grad_logp` and `entropy`
+        with `grad_entropy`.  `out` may be the scores themselves."""
+        scores_in, scores = scores, self._score_rows(scores)
+        n, k = scores.shape
+        ids = self._per_row(ids, "ids", torch.int64, n)
+        stats = self._per_row(stats, "stats", torch.float32, n, 2)
+        entropy = self._per_row(entropy, "entropy", torch.float32, n)
+        grad_logp = self._per_row(grad_logp, "grad_logp", torch.float32, n)
+        grad_entropy = self._per_row(grad_entropy, "grad_entropy", torch.float32, n)
+        if stats is None or (grad_logp is not None and ids is None) or (grad_entropy is not None and entropy is None):
+            raise ValueError("stats, ids with grad_logp, and entropy with grad_entropy are needed")
+        grad = self._grad_rows(out, scores_in)
+        if n:
+            check(lib.cd_log_probs_backward(self._h, _ptr(scores), SCORE_TYPES[scores.dtype], n, k,
+                                            self._row_stride(scores), float(temperature), _ptr(ids), _ptr(stats),
+                                            _ptr(entropy), _ptr(grad_logp), _ptr(grad_entropy), _ptr(grad),
+                                            self._row_stride(grad), self._stream()))
+        return grad
+
+    def _teacher(self, ids, scores, n):
+        self._check_dev(ids, "teacher_ids", torch.int64)
+        if ids.dim() != 2 or ids.shape[0] != n or not 1 <= ids.shape[1] <= 256:
+            raise ValueError(f"teacher_ids must be [{n}, 1..256], got {tuple(ids.shape)}")
+        if not torch.is_tensor(scores) or scores.device != self.device:
+            raise RuntimeError(f"teacher_scores must be a tensor on {self.device}")
+        if scores.dtype not in SCORE_TYPES:
+            raise TypeError(f"teacher_scores must be float32, bfloat16 or float16, got {scores.dtype}")
+        if scores.shape != ids.shape:
+            raise ValueError("teacher_scores and teacher_ids differ in shape")
+        return ids.contiguous(), scores.contiguous()
+
+    def distill(self, scores, teacher_ids, teacher_scores, weights=None, temperature=1.0, grad=False, out=None):
+        """Divergence of every row of scores (f32, bf16 or f16 [n, k]) from the distribution over a teacher's classes
+        teacher_ids (int64 [n, 1..256]; an id outside 0..k-1 is an unused entry) with teacher_scores of the same shape
+        (scores or log probabilities): `loss` [n] = weights * temperature^2 * KL(teacher || softmax(scores /
+        temperature)), `stats` [n, 2] for distill_backward and, with `grad`, `grad` [n, k]: the gradient of
+        loss.sum() in the scores' type, from the same pass (written to `out` if given, which may be the scores
+        themselves).  `weights` float32 [n]: rows of weight 0 are not read."""
+        scores_in, scores = scores, self._score_rows(scores)
+        n, k = scores.shape
+        teacher_ids, teacher_scores = self._teacher(teacher_ids, teacher_scores, n)
+        weights = self._per_row(weights, "weights", torch.float32, n)
+        if out is not None and not grad:
+            raise ValueError("out is for the gradient: pass grad=True")
+        res = {"loss": torch.empty((n,), dtype=torch.float32, device=self.device),
+               "stats": torch.empty((n, 2), dtype=torch.float32, device=self.device)}
+        if grad:
+            res["grad"] = self._grad_rows(out, scores_in)
+        if n:
+            ws, size = self._workspace(scores, 0)
+            check(lib.cd_distill(self._h, _ptr(scores), SCORE_TYPES[scores.dtype], n, k, self._row_stride(scores),
+                                 float(temperature), _ptr(teacher_ids), _ptr(teacher_scores),
+                                 SCORE_TYPES[teacher_scores.dtype], teacher_ids.shape[1], _ptr(weights),
+                                 _ptr(res["stats"]), _ptr(res["loss"]), _ptr(res.get("grad")),
+                                 self._row_stride(res["grad"]) if grad else 0, _ptr(ws), size, self._stream()))
+        return res
+
+    def distill_backward(self, scores, teacher_ids, teacher_scores, stats, grad_loss, weights=None, temperature=1.0,
+                         out=None):
+        """Gradient of sum(grad_loss * loss) with respect to the scores, from the `stats` of distill on the same
+        inputs.  `out` may be the scores themselves."""
+        scores_in, scores = scores, self._score_rows(scores)
+        n, k = scores.shape
+        teacher_ids, teacher_scores = self._teacher(teacher_ids, teacher_scores, n)
+        weights = self._per_row(weights, "weights", torch.float32, n)
+        stats = self._per_row(stats, "stats", torch.float32, n, 2)
+        grad_loss = self._per_row(grad_loss, "grad_loss", torch.float32, n)
+        if stats is None or grad_loss is None:
+            raise ValueError("stats and grad_loss are needed")
+        grad = self._grad_rows(out, scores_in)
+        if n:
+            check(lib.cd_distill_backward(self._h, _ptr(scores), SCORE_TYPES[scores.dtype], n, k,
+                                          self._row_stride(scores), float(temperature), _ptr(teacher_ids),
+                                          _ptr(teacher_scores), SCORE_TYPES[teacher_scores.dtype],
+                                          teacher_ids.shape[1], _ptr(weights), _ptr(stats), _ptr(grad_loss),
+                                          _ptr(grad), self._row_stride(grad), self._stream()))
+        return grad
 
     def rle(self, cls, maxv, frame_offset=0, cap=None):
         """Class stream -> dict of device tensors (end_frames, frame_types, run_lengths, start_frames,

@@ -245,6 +245,63 @@ int cd_eval_accumulate(cd_handle* h, const float* logits, const int64_t* labels,
                        int n_classes, int64_t* correct, int64_t* total, double* loss_sum,
                        void* stream);
 
+/* ---- Rows of class scores: log probabilities and distillation ------------------------------------------------
+ * The four calls below work on rows of scores in device memory, `n_classes` (1 .. 2^30) consecutive elements of
+ * `score_type` each, `row_stride` elements between the starts of two rows (0: every row is the same one), any
+ * alignment of the rows.  No counterpart in the reference, whose classifier ends at the scores.  z = x / temperature
+ * (2^-16 .. 2^16), p = softmax(z); the sums are held in 32 bits whatever the type.  A score of -inf has probability 0;
+ * a row of nothing but -inf has no distribution: log probabilities -inf, entropy 0, gradient 0.  A NaN or +inf makes
+ * its row's results NaN (the alternatives stay ordered as cd_max_argmax orders: NaN first).  A class id outside
+ * 0..n_classes-1 is skipped, as in cd_eval_accumulate.
+ * The calls use nothing of the handle but its device: they may overlap with other calls of the same handle, on any
+ * streams.  They allocate nothing and may be captured into a HIP graph; `workspace` (cd_rows_workspace bytes of device
+ * memory, 16-byte aligned; NULL where that is 0) holds values of one call only while that call's work runs.  Results do not depend on timing: two calls
+ * on the same inputs give the same bits. */
+enum { CD_T_F32 = 0, CD_T_BF16 = 1, CD_T_F16 = 2 };      /* element types of scores and their gradients */
+
+/* Bytes of device memory that cd_log_probs (`top` alternatives) or cd_distill (top = 0) needs beside its outputs for n
+ * rows; 0 for most sizes: only few, long rows are split between workgroups whose results meet there. */
+size_t cd_rows_workspace(int64_t n, int n_classes, int score_type, int top);
+
+/* Of every row the log probability of class ids[row] (logp f32 [n]; 0 where the id is skipped), the entropy
+ * -sum p ln p (entropy f32 [n]) and the `top` (0 .. 64, at most n_classes) classes with the highest scores and their
+ * log probabilities (top_ids i64, top_logp f32 [n][top]; equal scores in the order of their index).  stats f32 [n][2]:
+ * the row's largest score and sum exp(z - max z), for the backward call.  ids and logp may be NULL together, entropy
+ * may be NULL, top_ids and top_logp may be NULL with top = 0. */
+int cd_log_probs(cd_handle* h, const void* scores, int score_type, int64_t n, int n_classes, int64_t row_stride,
+                 float temperature, const int64_t* ids, int top, float* stats, float* logp, float* entropy,
+                 float* top_logp, int64_t* top_ids, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Gradient of sum over rows of grad_logp * logp + grad_entropy * entropy with respect to the scores, rounded once to
+ * their type: grad [n][n_classes], grad_stride elements (>= n_classes) between rows.  stats and entropy: of the forward
+ * call.  grad_logp (with ids) or grad_entropy (with entropy) may be NULL.  grad may be the scores' own memory with the
+ * scores' stride, and must not overlap with it otherwise. */
+int cd_log_probs_backward(cd_handle* h, const void* scores, int score_type, int64_t n, int n_classes,
+                          int64_t row_stride, float temperature, const int64_t* ids, const float* stats,
+                          const float* entropy, const float* grad_logp, const float* grad_entropy, void* grad,
+                          int64_t grad_stride, void* stream);
+
+/* Divergence of every row from a teacher's distribution over `entries` (1 .. 256) classes:
+ *   q = softmax(teacher_scores / temperature) over the row's entries, loss = w T^2 sum_j q_j (ln q_j - ln p[id_j])
+ * (T^2 keeps the gradient's size independent of the temperature).  teacher_ids i64 [n][entries]: an id outside
+ * 0..n_classes-1 marks an unused entry, whose score is not read; a class may be named more than once.  teacher_scores
+ * [n][entries] of teacher_type: scores or log probabilities, as cd_log_probs gives them (q does not depend on a constant
+ * added to a row).  weights f32 [n] or NULL (all 1): a row of weight 0 is not read, and its loss and gradient are 0, as
+ * are those of a row without used entries.  loss f32 [n]; stats f32 [n][2] as in cd_log_probs.
+ * grad: NULL, or [n][n_classes] of score_type for the gradient of the sum of the losses: w T (p - q), rounded once. May
+ * be the scores' own memory as in cd_log_probs_backward. */
+int cd_distill(cd_handle* h, const void* scores, int score_type, int64_t n, int n_classes, int64_t row_stride,
+               float temperature, const int64_t* teacher_ids, const void* teacher_scores, int teacher_type, int entries,
+               const float* weights, float* stats, float* loss, void* grad, int64_t grad_stride, void* workspace,
+               size_t workspace_bytes, void* stream);
+
+/* Gradient of sum over rows of grad_loss * loss, from the stats of the forward call: for losses that are combined
+ * further before they are differentiated.  Arguments as above. */
+int cd_distill_backward(cd_handle* h, const void* scores, int score_type, int64_t n, int n_classes, int64_t row_stride,
+                        float temperature, const int64_t* teacher_ids, const void* teacher_scores, int teacher_type,
+                        int entries, const float* weights, const float* stats, const float* grad_loss, void* grad,
+                        int64_t grad_stride, void* stream);
+
 /* Run-length encodes a per-frame class stream into segments.
  * Replaces frameID/segmentation.py:39-60 (Segmentation.__init__ after the max).
  * cls (i64 [n]) and maxv (f32 [n]) are device arrays.  Outputs are device arrays of capacity
