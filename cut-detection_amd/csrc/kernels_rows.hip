@@ -12,6 +12,7 @@
 // nothing but -inf has S = 0, log probability -inf everywhere, entropy 0 and gradient 0; a NaN or +inf among the
 // scores makes S, and with it the row's results, NaN.
 #include <algorithm>
+#include <cstdlib>
 
 #include "cd_internal.h"
 
@@ -32,7 +33,7 @@ typedef u32x4 __attribute__((aligned(2))) u32x4_any;      // 16 bytes at any ele
 
 template <int TYPE> struct Elem;
 template <> struct Elem<CD_T_F32> {
-    static constexpr int kVec = 4;
+    static constexpr int kVec = 4, kZeroBits = 0;        // (kZeroBits: low bits of a float that the type leaves 0)
     static constexpr uint32_t kNegInf = 0xff800000u;
     static __device__ __forceinline__ float load(const char* row, int64_t i) {
         return reinterpret_cast<const float*>(row)[i];
@@ -48,7 +49,7 @@ template <> struct Elem<CD_T_F32> {
     }
 };
 template <> struct Elem<CD_T_BF16> {
-    static constexpr int kVec = 8;
+    static constexpr int kVec = 8, kZeroBits = 16;
     static constexpr uint32_t kNegInf = 0xff80ff80u;
     static __device__ __forceinline__ float load(const char* row, int64_t i) {
         return __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(row)[i] << 16);
@@ -69,7 +70,7 @@ template <> struct Elem<CD_T_BF16> {
     }
 };
 template <> struct Elem<CD_T_F16> {
-    static constexpr int kVec = 8;
+    static constexpr int kVec = 8, kZeroBits = 13;
     static constexpr uint32_t kNegInf = 0xfc00fc00u;
     static __device__ __forceinline__ float load(const char* row, int64_t i) {
         return (float)reinterpret_cast<const _Float16*>(row)[i];
@@ -244,14 +245,40 @@ __device__ __forceinline__ void write_top(const LogProbsArgs& A, int64_t row, in
 }
 
 // ================================================================================== one workgroup per row
+// The highest classes of a row, from what the pass for the sums leaves behind.  The threads are 64 groups; the K-th
+// largest of the groups' maxima, T, is at most the K-th largest score, since K groups have a score that high.  Only
+// threads whose own maximum reaches T can hold one of the K highest: about K (1 + K / 128) of them for scores in no
+// particular order.  They read their scores again (from the caches), collect those that reach T in a list, and the list
+// is ranked by counting.  Scores equal to T may be very many (a mask): where a wave finds more than kDense threads at T
+// it leaves them, and the lowest-numbered classes at T are found by a scan in the order of the classes, which then ends
+// early.  A list that overflows all the same (scores laid out against the threads), and NaN, take one scan per class.
+constexpr int kDense = 24;
 template <int THREADS> struct BlockShared {
-    static constexpr int kWaves = THREADS / 64;
+    static constexpr int kWaves = THREADS / 64, kList = 1024;
     float m[kWaves], s[kWaves], u[kWaves];
+    uint32_t group[64];
+    int count, above, dense, part[kWaves];
+    uint8_t lane[kWaves][64];
     uint64_t key[kWaves];
+    uint64_t list[kList];
 };
 
+// the K-th largest of 64 lanes' keys
+template <int ZERO_BITS>
+__device__ __forceinline__ uint32_t kth_key(uint32_t key, int K) {
+    uint32_t t = 0;
+    const uint32_t part = key >> ZERO_BITS;
+    for (int b = 31 - ZERO_BITS; b >= 0; --b) {
+        const uint32_t up = t | 1u << b;
+        if (__popcll(__ballot(part >= up)) >= K) t = up;
+    }
+    t <<= ZERO_BITS;
+    return t & 0x80000000u ? t : t | ((1u << ZERO_BITS) - 1u);        // (keys of negative scores end in ones)
+}
+
+// The pass over a row; `mine` receives the maximum of the calling thread's scores.
 template <int TYPE, int THREADS, bool ENT>
-__device__ __forceinline__ Stat block_stat(const char* x, int k, float c, BlockShared<THREADS>& sh) {
+__device__ __forceinline__ Stat block_stat(const char* x, int k, float c, BlockShared<THREADS>& sh, float* mine) {
     using E = Elem<TYPE>;
     constexpr int U = 4, VE = E::kVec;
     const int nv = k / VE, tid = threadIdx.x;
@@ -271,9 +298,18 @@ __device__ __forceinline__ Stat block_stat(const char* x, int k, float c, BlockS
         const float xt = E::load(x, nv * VE + tid);
         accumulate<1, ENT>(&xt, a, c);
     }
+    *mine = a.m;
+    constexpr int G = THREADS / 64;                       // threads of a group
+    float g = a.m;
+    if (G > 1) g = fmaxf(g, dpp<0x111, 0xf>(-kInf, g));
+    if (G > 2) g = fmaxf(g, dpp<0x112, 0xf>(-kInf, g));
+    if (G > 4) g = fmaxf(g, dpp<0x114, 0xf>(-kInf, g));
+    if (G > 8) g = fmaxf(g, dpp<0x118, 0xf>(-kInf, g));
+    if (tid % G == G - 1) sh.group[tid / G] = score_key(g);
     a = wave_merge(a, c);
     const int wave = tid >> 6, lane = tid & 63;
     if (lane == 0) { sh.m[wave] = a.m; sh.s[wave] = a.s; sh.u[wave] = a.u; }
+    if (tid == 0) sh.count = sh.above = sh.dense = 0;
     __syncthreads();
     a.m = lane < THREADS / 64 ? sh.m[lane] : -kInf;
     a.s = lane < THREADS / 64 ? sh.s[lane] : 0.f;
@@ -281,29 +317,95 @@ __device__ __forceinline__ Stat block_stat(const char* x, int k, float c, BlockS
     return wave_merge(a, c);
 }
 
+// Calls emit(rank, key) for the K highest of the k scores, every rank once, by any thread.
+template <int TYPE, int THREADS, class Emit>
+__device__ __forceinline__ void block_top(const char* x, int k, int K, float mine, bool nan, BlockShared<THREADS>& sh,
+                                          Emit emit) {
+    using E = Elem<TYPE>;
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, nv = k / E::kVec;
+    const uint32_t T = kth_key<E::kZeroBits>(sh.group[lane], K);
+    if (!nan) {
+        const float xt = key_score(T);
+        auto collect = [&](float v, uint32_t i, bool ties) {
+            if (ties ? v >= xt : v > xt) {
+                const int at = atomicAdd(&sh.count, 1);
+                if (at < sh.kList) sh.list[at] = full_key(v, i);
+                if (v > xt) atomicAdd(&sh.above, 1);
+            }
+        };
+        const bool dense = __popcll(__ballot(mine == xt)) > kDense;
+        const uint64_t who = __ballot(dense ? mine > xt : mine >= xt);
+        if (dense && lane == 0) sh.dense = 1;
+        if (who >> lane & 1) sh.lane[wave][__popcll(who & ((1ull << lane) - 1))] = lane;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        const int share = (nv + THREADS - 1) / THREADS, items = __popcll(who) * share;
+        for (int it = lane; it < items; it += 64) {
+            const int q = it / share, v = (it - q * share) * THREADS + wave * 64 + sh.lane[wave][q];
+            if (v < nv) {
+                float xs[E::kVec];
+                E::unpack(reinterpret_cast<const u32x4_any*>(x)[v], xs);
+#pragma unroll
+                for (int i = 0; i < E::kVec; ++i) collect(xs[i], v * E::kVec + i, !dense);
+            }
+        }
+        const int i = nv * E::kVec + tid;
+        if (i < k) collect(E::load(x, i), i, !dense);
+    }
+    __syncthreads();
+    const int count = sh.count, above = sh.above, dense = sh.dense;
+    if (!nan && count <= sh.kList) {
+        for (int e = tid; e < count; e += THREADS) {
+            const uint64_t key = sh.list[e];
+            int rank = 0;
+            for (int j = 0; j < count; ++j) rank += sh.list[j] > key;
+            if (rank < K && (!dense || (uint32_t)(key >> 32) > T)) emit(rank, key);
+        }
+        for (int base = 0, rank = above; dense && rank < K && base < k; base += THREADS) {
+            const int i = base + tid;
+            const bool hit = i < k && score_key(E::load(x, i)) == T;
+            const uint64_t hits = __ballot(hit);
+            if (lane == 0) sh.part[wave] = __popcll(hits);
+            __syncthreads();
+            int before = 0, all = 0;
+            for (int w = 0; w < THREADS / 64; ++w) {
+                before += w < wave ? sh.part[w] : 0;
+                all += sh.part[w];
+            }
+            const int at = rank + before + __popcll(hits & ((1ull << lane) - 1));
+            if (hit && at < K) emit(at, (uint64_t)T << 32 | (uint32_t)~i);
+            rank += all;
+            __syncthreads();
+        }
+        return;
+    }
+    uint64_t last = ~0ull;
+    for (int r = 0; r < K; ++r) {                         // the largest key below the last one found
+        uint64_t best = 0;
+        for (int i = tid; i < k; i += THREADS) {
+            const uint64_t key = full_key(E::load(x, i), i);
+            if (key < last && key > best) best = key;
+        }
+        best = wave_max_key(best);
+        if (lane == 0) sh.key[wave] = best;
+        __syncthreads();
+        for (int w = 0; w < THREADS / 64; ++w) best = sh.key[w] > best ? sh.key[w] : best;
+        if (tid == 0) emit(r, best);
+        last = best;
+        __syncthreads();
+    }
+}
+
 template <int TYPE, int THREADS, bool ENT>
 __global__ __launch_bounds__(THREADS) void log_probs_block_kernel(LogProbsArgs A) {
     __shared__ BlockShared<THREADS> sh;
-    const int tid = threadIdx.x;
     for (int64_t row = blockIdx.x; row < A.n; row += gridDim.x) {
         const char* x = A.x + row * A.row_bytes;
-        const Stat a = block_stat<TYPE, THREADS, ENT>(x, A.k, A.c, sh);
-        if (tid == 0) write_row<TYPE>(A, row, x, a);
-        uint64_t last = ~0ull;
-        for (int r = 0; r < A.top; ++r) {                 // the largest key below the last one found
-            uint64_t best = 0;
-            for (int i = tid; i < A.k; i += THREADS) {
-                const uint64_t key = full_key(Elem<TYPE>::load(x, i), i);
-                if (key < last && key > best) best = key;
-            }
-            best = wave_max_key(best);
-            if ((tid & 63) == 0) sh.key[tid >> 6] = best;
-            __syncthreads();
-            for (int w = 0; w < THREADS / 64; ++w) best = sh.key[w] > best ? sh.key[w] : best;
-            if (tid == 0) write_top(A, row, r, best, a);
-            last = best;
-            __syncthreads();
-        }
+        float mine;
+        const Stat a = block_stat<TYPE, THREADS, ENT>(x, A.k, A.c, sh, &mine);
+        if (threadIdx.x == 0) write_row<TYPE>(A, row, x, a);
+        if (A.top)
+            block_top<TYPE>(x, A.k, A.top, mine, a.s != a.s, sh,
+                            [&](int rank, uint64_t key) { write_top(A, row, rank, key, a); });
         __syncthreads();
     }
 }
@@ -464,7 +566,8 @@ __global__ __launch_bounds__(THREADS) void distill_block_kernel(DistillArgs A) {
         te.total = 0.f;
         if (w != 0.f) {
             te = load_teacher<TYPE>(A, row, x);           // (every wave: the total decides for all of them)
-            a = block_stat<TYPE, THREADS, false>(x, A.k, A.c, sh);
+            float mine;
+            a = block_stat<TYPE, THREADS, false>(x, A.k, A.c, sh, &mine);
         }
         const bool on = w != 0.f && te.total != 0.f;
         if (tid < 64) {
@@ -542,6 +645,13 @@ __global__ __launch_bounds__(THREADS) void distill_grad_kernel(DistillGradArgs G
 constexpr int64_t kMaxGrid = 1 << 20;       // workgroups of a launch; further rows are taken by a loop
 unsigned row_grid(int64_t n) { return (unsigned)std::min(n, kMaxGrid); }
 
+int block_threads(const RowsIn& in) {
+#ifdef CD_EXP_ENV
+    if (const char* e = std::getenv("CUTDET_X_THREADS")) return std::atoi(e);
+#endif
+    return in.k > 32768 ? 1024 : 256;
+}
+
 #define CD_BY_TYPE(type, CALL)                       \
     do {                                             \
         if ((type) == CD_T_F32) { CALL(CD_T_F32); }  \
@@ -557,9 +667,15 @@ int launch_log_probs(const RowsIn& in, const int64_t* ids, int top, float* stats
                      float* top_logp, int64_t* top_ids, void* workspace, hipStream_t s) {
     const LogProbsArgs A = {static_cast<const char*>(in.x), in.n, in.stride * (in.type == CD_T_F32 ? 4 : 2), in.k, top,
                             kLog2e / in.temperature, in.temperature, ids, stats, logp, entropy, top_logp, top_ids};
+    const int threads = block_threads(in);
 #define CALL(TY)                                                                                                    \
-    if (entropy) log_probs_block_kernel<TY, 256, true><<<row_grid(in.n), 256, 0, s>>>(A);                           \
-    else log_probs_block_kernel<TY, 256, false><<<row_grid(in.n), 256, 0, s>>>(A)
+    if (threads == 1024) {                                                                                          \
+        if (entropy) log_probs_block_kernel<TY, 1024, true><<<row_grid(in.n), 1024, 0, s>>>(A);                     \
+        else log_probs_block_kernel<TY, 1024, false><<<row_grid(in.n), 1024, 0, s>>>(A);                            \
+    } else {                                                                                                        \
+        if (entropy) log_probs_block_kernel<TY, 256, true><<<row_grid(in.n), 256, 0, s>>>(A);                       \
+        else log_probs_block_kernel<TY, 256, false><<<row_grid(in.n), 256, 0, s>>>(A);                              \
+    }
     CD_BY_TYPE(in.type, CALL);
 #undef CALL
     CD_HIP(hipGetLastError());
@@ -589,7 +705,10 @@ static DistillArgs distill_args(const RowsIn& in, const TeacherIn& te, float* st
 int launch_distill(const RowsIn& in, const TeacherIn& te, float* stats, float* loss, void* dx, int64_t dx_stride,
                    void* workspace, hipStream_t s) {
     const DistillArgs A = distill_args(in, te, stats, loss, dx, dx_stride);
-#define CALL(TY) distill_block_kernel<TY, 256><<<row_grid(in.n), 256, 0, s>>>(A)
+    const int threads = block_threads(in);
+#define CALL(TY)                                                                                   \
+    if (threads == 1024) distill_block_kernel<TY, 1024><<<row_grid(in.n), 1024, 0, s>>>(A);        \
+    else distill_block_kernel<TY, 256><<<row_grid(in.n), 256, 0, s>>>(A)
     CD_BY_TYPE(in.type, CALL);
 #undef CALL
     CD_HIP(hipGetLastError());
