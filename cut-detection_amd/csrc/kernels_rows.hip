@@ -474,25 +474,23 @@ struct DistillArgs {
     float c, t;
     const int64_t* ids;
     const void* teacher;
-    const float *weights;
+    const float *weights, *g_loss;  // g_loss: only the gradient, each row's times g_loss
     float *stats, *loss;
 };
-constexpr int kTeacherPerLane = kMaxTeacher / 64;
-
-struct Teacher {                    // the entries of one row, spread over a wave: entry lane + 64 e
-    int id[kTeacherPerLane];        // -1: unused
-    float lq[kTeacherPerLane];      // log2 q
-    float q[kTeacherPerLane];       // its share; after `share` of the first entry of a class the sum over its entries
-    float x[kTeacherPerLane];       // the student's score
+template <int PER> struct Teacher { // the entries of one row, spread over a wave: entry lane + 64 e, e < PER
+    int id[PER];                    // -1: unused
+    float lq[PER];                  // log2 q
+    float q[PER];
+    float x[PER];                   // the student's score
     float total;                    // sum of 2^(..) before normalising: 0 where no entry counts
 };
-template <int TYPE>
-__device__ __forceinline__ Teacher load_teacher(const DistillArgs& A, int64_t row, const char* x) {
-    Teacher r;
+template <int TYPE, int PER>
+__device__ __forceinline__ Teacher<PER> load_teacher(const DistillArgs& A, int64_t row, const char* x) {
+    Teacher<PER> r;
     const int lane = threadIdx.x & 63;
     float m = -kInf;
 #pragma unroll
-    for (int e = 0; e < kTeacherPerLane; ++e) {
+    for (int e = 0; e < PER; ++e) {
         const int j = lane + 64 * e;
         int64_t id = -1;
         float v = -kInf;
@@ -508,7 +506,7 @@ __device__ __forceinline__ Teacher load_teacher(const DistillArgs& A, int64_t ro
     const Ref t_of(m, A.c);
     float total = 0.f;
 #pragma unroll
-    for (int e = 0; e < kTeacherPerLane; ++e) {
+    for (int e = 0; e < PER; ++e) {
         r.lq[e] = t_of(r.lq[e]);
         r.q[e] = r.id[e] >= 0 ? __builtin_amdgcn_exp2f(r.lq[e]) : 0.f;
         total += r.q[e];
@@ -516,43 +514,50 @@ __device__ __forceinline__ Teacher load_teacher(const DistillArgs& A, int64_t ro
     r.total = wave_sum(total);
     const float l = __builtin_amdgcn_logf(r.total), inv = 1.f / r.total;
 #pragma unroll
-    for (int e = 0; e < kTeacherPerLane; ++e) { r.lq[e] -= l; r.q[e] *= inv; }
+    for (int e = 0; e < PER; ++e) { r.lq[e] -= l; r.q[e] *= inv; }
     return r;
 }
+// one entry's part of a loss of weight and temperature 1
+__device__ __forceinline__ float loss_term(float q, float lq, float x, const Stat& a, float c, float temperature) {
+    return q != 0.f ? q * (kLn2 * lq - logp_of(x, a, c, temperature)) : 0.f;
+}
 // the row's loss, uniform over the wave
-__device__ __forceinline__ float teacher_loss(const Teacher& r, const Stat& a, const DistillArgs& A, float w) {
+template <int PER>
+__device__ __forceinline__ float teacher_loss(const Teacher<PER>& r, const Stat& a, const DistillArgs& A, float w) {
     float sum = 0.f;
 #pragma unroll
-    for (int e = 0; e < kTeacherPerLane; ++e)
-        if (r.id[e] >= 0 && r.q[e] != 0.f)
-            sum = __builtin_fmaf(r.q[e], kLn2 * r.lq[e] - logp_of(r.x[e], a, A.c, A.t), sum);
+    for (int e = 0; e < PER; ++e)
+        if (r.id[e] >= 0) sum += loss_term(r.q[e], r.lq[e], r.x[e], a, A.c, A.t);
     return w * (A.t * A.t) * wave_sum(sum);
 }
 // gradient at the teacher's classes: of a class named twice the first entry has the sum, the others none
-template <int TYPE>
-__device__ __forceinline__ void fix_gradient(const Teacher& r, const Stat& a, const DistillArgs& A, float w, char* dx) {
+template <int TYPE, int PER>
+__device__ __forceinline__ void fix_gradient(const Teacher<PER>& r, const Stat& a, const DistillArgs& A, float w, char* dx) {
     const Ref t_of(a.m, A.c);
     const float inv = 1.f / a.s;
     const int lane = threadIdx.x & 63;
+    float sum[PER];
+    bool first[PER];
 #pragma unroll
-    for (int e = 0; e < kTeacherPerLane; ++e) {
-        float sum = 0.f;
-        bool first = r.id[e] >= 0;
+    for (int e = 0; e < PER; ++e) { sum[e] = 0.f; first[e] = r.id[e] >= 0; }
 #pragma unroll
-        for (int f = 0; f < kTeacherPerLane; ++f)
-            for (int l = 0; l < min(64, A.entries - 64 * f); ++l) {
-                const int id = __builtin_amdgcn_readlane(r.id[f], l);
-                const float q = lane_of(r.q[f], l);
+    for (int f = 0; f < PER; ++f)
+        for (int l = 0; l < min(64, A.entries - 64 * f); ++l) {
+            const int id = __builtin_amdgcn_readlane(r.id[f], l);
+            const float q = lane_of(r.q[f], l);
+#pragma unroll
+            for (int e = 0; e < PER; ++e)
                 if (id == r.id[e]) {
-                    sum += q;
-                    if (64 * f + l < 64 * e + lane) first = false;
+                    sum[e] += q;
+                    if (64 * f + l < 64 * e + lane) first[e] = false;
                 }
-            }
-        if (first) Elem<TYPE>::store(dx, r.id[e], w * A.t * (__builtin_amdgcn_exp2f(t_of(r.x[e])) * inv - sum));
-    }
+        }
+#pragma unroll
+    for (int e = 0; e < PER; ++e)
+        if (first[e]) Elem<TYPE>::store(dx, r.id[e], w * A.t * (__builtin_amdgcn_exp2f(t_of(r.x[e])) * inv - sum[e]));
 }
 
-template <int TYPE, int THREADS>
+template <int TYPE, int THREADS, int PER>
 __global__ __launch_bounds__(THREADS) void distill_block_kernel(DistillArgs A) {
     using E = Elem<TYPE>;
     __shared__ BlockShared<THREADS> sh;
@@ -562,10 +567,10 @@ __global__ __launch_bounds__(THREADS) void distill_block_kernel(DistillArgs A) {
         char* dx = A.dx + row * A.dx_row_bytes;
         const float w = A.weights ? A.weights[row] : 1.f;
         Stat a = {-kInf, 0.f, 0.f};
-        Teacher te;
+        Teacher<PER> te;
         te.total = 0.f;
         if (w != 0.f) {
-            te = load_teacher<TYPE>(A, row, x);           // (every wave: the total decides for all of them)
+            te = load_teacher<TYPE, PER>(A, row, x);           // (every wave: the total decides for all of them)
             float mine;
             a = block_stat<TYPE, THREADS, false>(x, A.k, A.c, sh, &mine);
         }
@@ -595,31 +600,26 @@ __global__ __launch_bounds__(THREADS) void distill_block_kernel(DistillArgs A) {
             const int i = nv * E::kVec + tid;
             if (i < A.k) E::store(dx, i, live ? f * __builtin_amdgcn_exp2f(t_of(E::load(x, i))) : 0.f);
             __syncthreads();
-            if (live && tid < 64) fix_gradient<TYPE>(te, a, A, w, dx);
+            if (live && tid < 64) fix_gradient<TYPE, PER>(te, a, A, w, dx);
         }
         __syncthreads();
     }
 }
 
 // the gradient alone, for a loss gradient g per row, from the statistics of the forward call
-struct DistillGradArgs {
-    DistillArgs d;
-    const float* g_loss;
-};
-template <int TYPE, int THREADS>
-__global__ __launch_bounds__(THREADS) void distill_grad_kernel(DistillGradArgs G) {
+template <int TYPE, int THREADS, int PER>
+__global__ __launch_bounds__(THREADS) void distill_grad_kernel(DistillArgs A) {
     using E = Elem<TYPE>;
-    const DistillArgs& A = G.d;
     const int tid = threadIdx.x;
     for (int64_t row = blockIdx.x; row < A.n; row += gridDim.x) {
         const char* x = A.x + row * A.row_bytes;
         char* dx = A.dx + row * A.dx_row_bytes;
         const float w = (A.weights ? A.weights[row] : 1.f);
-        const float wg = w == 0.f ? 0.f : w * G.g_loss[row];
+        const float wg = w == 0.f ? 0.f : w * A.g_loss[row];
         const Stat a = {A.stats[2 * row], A.stats[2 * row + 1], 0.f};
-        Teacher te;
+        Teacher<PER> te;
         te.total = 0.f;
-        if (wg != 0.f) te = load_teacher<TYPE>(A, row, x);
+        if (wg != 0.f) te = load_teacher<TYPE, PER>(A, row, x);
         __syncthreads();                                  // dx may be x: the teacher's classes are read before any write
         const bool live = wg != 0.f && te.total != 0.f && a.s != 0.f;
         const Ref t_of(a.m, A.c);
@@ -637,8 +637,246 @@ __global__ __launch_bounds__(THREADS) void distill_grad_kernel(DistillGradArgs G
         const int i = nv * E::kVec + tid;
         if (i < A.k) E::store(dx, i, live ? f * __builtin_amdgcn_exp2f(t_of(E::load(x, i))) : 0.f);
         __syncthreads();
-        if (live && tid < 64) fix_gradient<TYPE>(te, a, A, wg, dx);
+        if (live && tid < 64) fix_gradient<TYPE, PER>(te, a, A, wg, dx);
         __syncthreads();
+    }
+}
+
+// ================================================================================== one thread per row, up to 16 scores
+constexpr int kThreadClasses = 16;
+
+template <int TYPE, int K>
+__device__ __forceinline__ void load_short(const char* x, int k, float* v) {
+#pragma unroll
+    for (int i = 0; i < K; ++i) v[i] = i < k ? Elem<TYPE>::load(x, i) : -kInf;
+}
+
+template <int TYPE, int K>
+__global__ __launch_bounds__(64) void log_probs_thread_kernel(LogProbsArgs A) {
+    for (int64_t row = (int64_t)blockIdx.x * 64 + threadIdx.x; row < A.n; row += (int64_t)gridDim.x * 64) {
+        const char* x = A.x + row * A.row_bytes;
+        float v[K];
+        load_short<TYPE, K>(x, A.k, v);
+        Stat a = {-kInf, 0.f, 0.f};
+        accumulate<K, true>(v, a, A.c);
+        write_row<TYPE>(A, row, x, a);
+        uint32_t key[K], used = 0;
+#pragma unroll
+        for (int i = 0; i < K; ++i) key[i] = score_key(v[i]);
+        for (int r = 0; r < A.top; ++r) {
+            uint32_t best = 0;
+            int at = 0;
+#pragma unroll
+            for (int i = 0; i < K; ++i)
+                if (i < A.k && !(used >> i & 1) && key[i] > best) { best = key[i]; at = i; }
+            used |= 1u << at;
+            write_top(A, row, r, (uint64_t)best << 32 | (uint32_t)~at, a);
+        }
+    }
+}
+
+template <int TYPE, int K>
+__global__ __launch_bounds__(64) void log_probs_grad_thread_kernel(LogProbsGradArgs A) {
+    for (int64_t row = (int64_t)blockIdx.x * 64 + threadIdx.x; row < A.n; row += (int64_t)gridDim.x * 64) {
+        const float m = A.stats[2 * row], s = A.stats[2 * row + 1];
+        float v[K];
+        load_short<TYPE, K>(A.x + row * A.row_bytes, A.k, v);
+        const GradRow g = grad_row(A, row, s);
+        const Ref t_of(m, A.c);
+#pragma unroll
+        for (int i = 0; i < K; ++i)
+            if (i < A.k)
+                Elem<TYPE>::store(A.dx + row * A.dx_row_bytes, i, grad_of(t_of(v[i]), g) + (i == g.id ? g.hit : 0.f));
+    }
+}
+
+template <int TYPE, int K>
+__global__ __launch_bounds__(64) void distill_thread_kernel(DistillArgs A) {
+    for (int64_t row = (int64_t)blockIdx.x * 64 + threadIdx.x; row < A.n; row += (int64_t)gridDim.x * 64) {
+        const char* x = A.x + row * A.row_bytes;
+        float w = A.weights ? A.weights[row] : 1.f;
+        if (A.g_loss && w != 0.f) w *= A.g_loss[row];
+        float v[K], qk[K], loss = 0.f, total = 0.f;
+        Stat a = {-kInf, 0.f, 0.f};
+        if (w != 0.f) {
+            load_short<TYPE, K>(x, A.k, v);
+            accumulate<K, false>(v, a, A.c);
+            const int64_t* ids = A.ids + row * A.entries;
+            auto used = [&](int64_t id) { return id >= 0 && id < A.k; };
+            auto score = [&](int j) { return load_any(A.teacher_type, A.teacher, row * A.entries + j); };
+            float m = -kInf;
+            for (int j = 0; j < A.entries; ++j) if (used(ids[j])) m = fmaxf(m, score(j));
+            const Ref t_of(m, A.c);
+            for (int j = 0; j < A.entries; ++j) if (used(ids[j])) total += __builtin_amdgcn_exp2f(t_of(score(j)));
+            const float l = __builtin_amdgcn_logf(total), inv = 1.f / total;
+#pragma unroll
+            for (int i = 0; i < K; ++i) qk[i] = 0.f;
+            if (total != 0.f)
+                for (int j = 0; j < A.entries; ++j) {
+                    const int64_t id = ids[j];
+                    if (!used(id)) continue;
+                    const float t = t_of(score(j)), q = __builtin_amdgcn_exp2f(t) * inv;
+                    float xj = 0.f;
+#pragma unroll
+                    for (int i = 0; i < K; ++i) if (i == id) { xj = v[i]; qk[i] += q; }
+                    loss += loss_term(q, t - l, xj, a, A.c, A.t);
+                }
+        }
+        const bool on = w != 0.f && total != 0.f, live = on && a.s != 0.f;
+        if (A.loss) {
+            A.loss[row] = on ? w * (A.t * A.t) * loss : 0.f;
+            A.stats[2 * row] = a.m;
+            A.stats[2 * row + 1] = a.s;
+        }
+        if (A.dx) {
+            const Ref t_of(a.m, A.c);
+            const float inv = 1.f / a.s;
+#pragma unroll
+            for (int i = 0; i < K; ++i)
+                if (i < A.k)
+                    Elem<TYPE>::store(A.dx + row * A.dx_row_bytes, i,
+                                      live ? w * A.t * (__builtin_amdgcn_exp2f(t_of(v[i])) * inv - qk[i]) : 0.f);
+        }
+    }
+}
+
+// ================================================================================== one wave per row, up to 1024 scores
+// Score i is in lane i % 64, so the order of the classes is the order of (register, lane).
+constexpr int kWaveClasses = 1024;
+
+template <int TYPE, int N>
+__device__ __forceinline__ void load_spread(const char* x, int k, float* v) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = lane + 64 * j < k ? Elem<TYPE>::load(x, lane + 64 * j) : -kInf;
+}
+
+// As block_top; where more than 64 scores reach T (equal ones), the K-th largest score itself takes the place of T, and
+// of those equal to it the lowest classes count.
+template <int TYPE, int N, class Emit>
+__device__ __forceinline__ void wave_top(const float* v, int k, int K, float mine, bool nan, uint64_t* list, Emit emit) {
+    const int lane = threadIdx.x & 63;
+    const uint64_t below = (1ull << lane) - 1;
+    uint32_t key[N], high = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) key[j] = lane + 64 * j < k ? score_key(v[j]) : 0;
+    if (nan) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) high = key[j] > high ? key[j] : high;
+    } else if (lane < k) high = score_key(mine);
+    uint32_t t = kth_key<0>(high, K);
+    int count = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) count += __popcll(__ballot(key[j] >= t));
+    int ties = 64;                                        // of the scores at t, as many as there are
+    if (count > 64) {
+        t = 0;
+        for (int b = 31; b >= 0; --b) {
+            const uint32_t up = t | 1u << b;
+            int c = 0;
+#pragma unroll
+            for (int j = 0; j < N; ++j) c += __popcll(__ballot(key[j] >= up));
+            if (c >= K) t = up;
+        }
+        int above = 0;
+#pragma unroll
+        for (int j = 0; j < N; ++j) above += __popcll(__ballot(key[j] > t));
+        ties = K - above;
+    }
+    count = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const uint64_t equal = __ballot(key[j] == t), up = __ballot(key[j] > t);
+        const bool take = up >> lane & 1 || (equal >> lane & 1 && __popcll(equal & below) < ties);
+        const uint64_t taken = __ballot(take);
+        if (take) list[count + __popcll(taken & below)] = (uint64_t)key[j] << 32 | (uint32_t)~(lane + 64 * j);
+        count += __popcll(taken);
+        ties -= min(ties, __popcll(equal));
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (lane < count) {
+        const uint64_t mykey = list[lane];
+        int rank = 0;
+        for (int j = 0; j < count; ++j) rank += list[j] > mykey;
+        if (rank < K) emit(rank, mykey);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+}
+
+template <int TYPE, int N, bool ENT>
+__global__ __launch_bounds__(256) void log_probs_wave_kernel(LogProbsArgs A) {
+    __shared__ uint64_t list[4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int64_t row = (int64_t)blockIdx.x * 4 + wave; row < A.n; row += (int64_t)gridDim.x * 4) {
+        const char* x = A.x + row * A.row_bytes;
+        float v[N];
+        load_spread<TYPE, N>(x, A.k, v);
+        Stat a = {-kInf, 0.f, 0.f};
+        accumulate<N, ENT>(v, a, A.c);
+        const float mine = a.m;
+        a = wave_merge(a, A.c);
+        if (lane == 0) write_row<TYPE>(A, row, x, a);
+        if (A.top)
+            wave_top<TYPE, N>(v, A.k, A.top, mine, a.s != a.s, list[wave],
+                              [&](int rank, uint64_t key) { write_top(A, row, rank, key, a); });
+    }
+}
+
+template <int TYPE, int N>
+__global__ __launch_bounds__(256) void log_probs_grad_wave_kernel(LogProbsGradArgs A) {
+    const int lane = threadIdx.x & 63;
+    for (int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); row < A.n; row += (int64_t)gridDim.x * 4) {
+        const float m = A.stats[2 * row], s = A.stats[2 * row + 1];
+        float v[N];
+        load_spread<TYPE, N>(A.x + row * A.row_bytes, A.k, v);
+        const GradRow g = grad_row(A, row, s);
+        const Ref t_of(m, A.c);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int i = lane + 64 * j;
+            if (i < A.k)
+                Elem<TYPE>::store(A.dx + row * A.dx_row_bytes, i, grad_of(t_of(v[j]), g) + (i == g.id ? g.hit : 0.f));
+        }
+    }
+}
+
+template <int TYPE, int N, int PER>
+__global__ __launch_bounds__(256) void distill_wave_kernel(DistillArgs A) {
+    const int lane = threadIdx.x & 63;
+    for (int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); row < A.n; row += (int64_t)gridDim.x * 4) {
+        const char* x = A.x + row * A.row_bytes;
+        char* dx = A.dx + row * A.dx_row_bytes;
+        float w = A.weights ? A.weights[row] : 1.f;
+        if (A.g_loss && w != 0.f) w *= A.g_loss[row];
+        float v[N];
+        Stat a = {-kInf, 0.f, 0.f};
+        Teacher<PER> te;
+        te.total = 0.f;
+        if (w != 0.f) {
+            load_spread<TYPE, N>(x, A.k, v);
+            te = load_teacher<TYPE, PER>(A, row, x);
+            accumulate<N, false>(v, a, A.c);
+            a = wave_merge(a, A.c);
+        }
+        const bool on = w != 0.f && te.total != 0.f, live = on && a.s != 0.f;
+        if (A.loss) {
+            const float loss = on ? teacher_loss<PER>(te, a, A, w) : 0.f;
+            if (lane == 0) {
+                A.loss[row] = loss;
+                A.stats[2 * row] = a.m;
+                A.stats[2 * row + 1] = a.s;
+            }
+        }
+        if (A.dx) {
+            const Ref t_of(a.m, A.c);
+            const float f = live ? w * A.t / a.s : 0.f;
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                if (lane + 64 * j < A.k)
+                    Elem<TYPE>::store(dx, lane + 64 * j, live ? f * __builtin_amdgcn_exp2f(t_of(v[j])) : 0.f);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");      // the row first, then the teacher's classes
+            if (live) fix_gradient<TYPE, PER>(te, a, A, w, dx);
+        }
     }
 }
 
@@ -652,12 +890,17 @@ int block_threads(const RowsIn& in) {
     return in.k > 32768 ? 1024 : 256;
 }
 
-#define CD_BY_TYPE(type, CALL)                       \
-    do {                                             \
-        if ((type) == CD_T_F32) { CALL(CD_T_F32); }  \
-        else if ((type) == CD_T_BF16) { CALL(CD_T_BF16); } \
-        else { CALL(CD_T_F16); }                     \
+// CALL(type, ...) for the type of the scores
+#define CD_BY_TYPE(type, CALL, ...)                                     \
+    do {                                                                \
+        if ((type) == CD_T_F32) { CALL(CD_T_F32, __VA_ARGS__); }        \
+        else if ((type) == CD_T_BF16) { CALL(CD_T_BF16, __VA_ARGS__); } \
+        else { CALL(CD_T_F16, __VA_ARGS__); }                           \
     } while (0)
+
+unsigned thread_grid(int64_t n) { return row_grid((n + 63) / 64); }
+unsigned wave_grid(int64_t n) { return row_grid((n + 3) / 4); }
+int elem_size(int type) { return type == CD_T_F32 ? 4 : 2; }
 
 }  // namespace
 
@@ -665,62 +908,99 @@ size_t rows_workspace(int64_t n, int k, int type, int top) { return 0; }
 
 int launch_log_probs(const RowsIn& in, const int64_t* ids, int top, float* stats, float* logp, float* entropy,
                      float* top_logp, int64_t* top_ids, void* workspace, hipStream_t s) {
-    const LogProbsArgs A = {static_cast<const char*>(in.x), in.n, in.stride * (in.type == CD_T_F32 ? 4 : 2), in.k, top,
+    const LogProbsArgs A = {static_cast<const char*>(in.x), in.n, in.stride * elem_size(in.type), in.k, top,
                             kLog2e / in.temperature, in.temperature, ids, stats, logp, entropy, top_logp, top_ids};
-    const int threads = block_threads(in);
-#define CALL(TY)                                                                                                    \
-    if (threads == 1024) {                                                                                          \
-        if (entropy) log_probs_block_kernel<TY, 1024, true><<<row_grid(in.n), 1024, 0, s>>>(A);                     \
-        else log_probs_block_kernel<TY, 1024, false><<<row_grid(in.n), 1024, 0, s>>>(A);                            \
-    } else {                                                                                                        \
-        if (entropy) log_probs_block_kernel<TY, 256, true><<<row_grid(in.n), 256, 0, s>>>(A);                       \
-        else log_probs_block_kernel<TY, 256, false><<<row_grid(in.n), 256, 0, s>>>(A);                              \
-    }
-    CD_BY_TYPE(in.type, CALL);
-#undef CALL
+#define SHORT(TY, K) log_probs_thread_kernel<TY, K><<<thread_grid(in.n), 64, 0, s>>>(A)
+#define WAVE(TY, N)                                                                         \
+    if (entropy) log_probs_wave_kernel<TY, N, true><<<wave_grid(in.n), 256, 0, s>>>(A);     \
+    else log_probs_wave_kernel<TY, N, false><<<wave_grid(in.n), 256, 0, s>>>(A)
+#define BLOCK(TY, TH)                                                                       \
+    if (entropy) log_probs_block_kernel<TY, TH, true><<<row_grid(in.n), TH, 0, s>>>(A);     \
+    else log_probs_block_kernel<TY, TH, false><<<row_grid(in.n), TH, 0, s>>>(A)
+    if (in.k <= 4) CD_BY_TYPE(in.type, SHORT, 4);
+    else if (in.k <= kThreadClasses) CD_BY_TYPE(in.type, SHORT, kThreadClasses);
+    else if (in.k <= 256) CD_BY_TYPE(in.type, WAVE, 4);
+    else if (in.k <= kWaveClasses) CD_BY_TYPE(in.type, WAVE, 16);
+    else if (block_threads(in) == 256) CD_BY_TYPE(in.type, BLOCK, 256);
+    else CD_BY_TYPE(in.type, BLOCK, 1024);
+#undef SHORT
+#undef WAVE
+#undef BLOCK
     CD_HIP(hipGetLastError());
     return CD_OK;
 }
 
 int launch_log_probs_backward(const RowsIn& in, const int64_t* ids, const float* stats, const float* entropy,
                               const float* g_logp, const float* g_entropy, void* dx, int64_t dx_stride, hipStream_t s) {
-    const int size = in.type == CD_T_F32 ? 4 : 2;
+    const int size = elem_size(in.type);
     const LogProbsGradArgs A = {static_cast<const char*>(in.x), static_cast<char*>(dx), in.n, in.stride * size,
                                 dx_stride * size, in.k, kLog2e / in.temperature, 1.f / in.temperature, ids, stats,
                                 entropy, g_logp, g_entropy};
-#define CALL(TY) log_probs_grad_kernel<TY, 256><<<row_grid(in.n), 256, 0, s>>>(A)
-    CD_BY_TYPE(in.type, CALL);
-#undef CALL
+#define SHORT(TY, K) log_probs_grad_thread_kernel<TY, K><<<thread_grid(in.n), 64, 0, s>>>(A)
+#define WAVE(TY, N) log_probs_grad_wave_kernel<TY, N><<<wave_grid(in.n), 256, 0, s>>>(A)
+#define BLOCK(TY, TH) log_probs_grad_kernel<TY, TH><<<row_grid(in.n), TH, 0, s>>>(A)
+    if (in.k <= 4) CD_BY_TYPE(in.type, SHORT, 4);
+    else if (in.k <= kThreadClasses) CD_BY_TYPE(in.type, SHORT, kThreadClasses);
+    else if (in.k <= 256) CD_BY_TYPE(in.type, WAVE, 4);
+    else if (in.k <= kWaveClasses) CD_BY_TYPE(in.type, WAVE, 16);
+    else CD_BY_TYPE(in.type, BLOCK, 256);
+#undef SHORT
+#undef WAVE
+#undef BLOCK
     CD_HIP(hipGetLastError());
     return CD_OK;
 }
 
-static DistillArgs distill_args(const RowsIn& in, const TeacherIn& te, float* stats, float* loss, void* dx,
-                                int64_t dx_stride) {
-    const int size = in.type == CD_T_F32 ? 4 : 2;
+static DistillArgs distill_args(const RowsIn& in, const TeacherIn& te, float* stats, float* loss, const float* g_loss,
+                                void* dx, int64_t dx_stride) {
+    const int size = elem_size(in.type);
     return {static_cast<const char*>(in.x), static_cast<char*>(dx), in.n, in.stride * size, dx_stride * size, in.k,
-            te.entries, te.type, kLog2e / in.temperature, in.temperature, te.ids, te.scores, te.weights, stats, loss};
+            te.entries, te.type, kLog2e / in.temperature, in.temperature, te.ids, te.scores, te.weights, g_loss, stats,
+            loss};
+}
+
+// rows of up to kWaveClasses scores, which the gradient alone computes anew; false: longer ones
+static bool launch_short_distill(const RowsIn& in, const DistillArgs& A, hipStream_t s) {
+#define SHORT(TY, K) distill_thread_kernel<TY, K><<<thread_grid(in.n), 64, 0, s>>>(A)
+#define WAVE(TY, N)                                                                                \
+    if (A.entries <= 64) distill_wave_kernel<TY, N, 1><<<wave_grid(in.n), 256, 0, s>>>(A);         \
+    else distill_wave_kernel<TY, N, kMaxTeacher / 64><<<wave_grid(in.n), 256, 0, s>>>(A)
+    if (in.k <= 4 && A.entries <= 16) CD_BY_TYPE(in.type, SHORT, 4);
+    else if (in.k <= kThreadClasses && A.entries <= 16) CD_BY_TYPE(in.type, SHORT, kThreadClasses);
+    else if (in.k <= 256) CD_BY_TYPE(in.type, WAVE, 4);
+    else if (in.k <= kWaveClasses) CD_BY_TYPE(in.type, WAVE, 16);
+    else return false;
+#undef SHORT
+#undef WAVE
+    return true;
 }
 
 int launch_distill(const RowsIn& in, const TeacherIn& te, float* stats, float* loss, void* dx, int64_t dx_stride,
                    void* workspace, hipStream_t s) {
-    const DistillArgs A = distill_args(in, te, stats, loss, dx, dx_stride);
-    const int threads = block_threads(in);
-#define CALL(TY)                                                                                   \
-    if (threads == 1024) distill_block_kernel<TY, 1024><<<row_grid(in.n), 1024, 0, s>>>(A);        \
-    else distill_block_kernel<TY, 256><<<row_grid(in.n), 256, 0, s>>>(A)
-    CD_BY_TYPE(in.type, CALL);
-#undef CALL
+    const DistillArgs A = distill_args(in, te, stats, loss, nullptr, dx, dx_stride);
+    if (!launch_short_distill(in, A, s)) {
+#define BLOCK(TY, TH)                                                                                       \
+    if (A.entries <= 64) distill_block_kernel<TY, TH, 1><<<row_grid(in.n), TH, 0, s>>>(A);                  \
+    else distill_block_kernel<TY, TH, kMaxTeacher / 64><<<row_grid(in.n), TH, 0, s>>>(A)
+        if (block_threads(in) == 256) CD_BY_TYPE(in.type, BLOCK, 256);
+        else CD_BY_TYPE(in.type, BLOCK, 1024);
+#undef BLOCK
+    }
     CD_HIP(hipGetLastError());
     return CD_OK;
 }
 
 int launch_distill_backward(const RowsIn& in, const TeacherIn& te, const float* stats, const float* g_loss, void* dx,
                             int64_t dx_stride, hipStream_t s) {
-    const DistillGradArgs G = {distill_args(in, te, const_cast<float*>(stats), nullptr, dx, dx_stride), g_loss};
-#define CALL(TY) distill_grad_kernel<TY, 256><<<row_grid(in.n), 256, 0, s>>>(G)
-    CD_BY_TYPE(in.type, CALL);
-#undef CALL
+    DistillArgs A = distill_args(in, te, nullptr, nullptr, g_loss, dx, dx_stride);
+    if (!launch_short_distill(in, A, s)) {
+        A.stats = const_cast<float*>(stats);              // only read
+#define BLOCK(TY, TH)                                                                                       \
+    if (A.entries <= 64) distill_grad_kernel<TY, TH, 1><<<row_grid(in.n), TH, 0, s>>>(A);                   \
+    else distill_grad_kernel<TY, TH, kMaxTeacher / 64><<<row_grid(in.n), TH, 0, s>>>(A)
+        CD_BY_TYPE(in.type, BLOCK, 256);
+#undef BLOCK
+    }
     CD_HIP(hipGetLastError());
     return CD_OK;
 }

@@ -4,6 +4,7 @@ PyTorch supplies device memory and the current HIP stream; every operation is on
 libcutdet.so.  Inputs must live on the engine's GPU -- there is no CPU path.
 """
 import ctypes as C
+import functools
 
 import torch
 
@@ -31,7 +32,12 @@ def sampled_source_rows(height, width, resize=NET_W):
 
 
 def _ptr(t):
-    return C.c_void_p(t.data_ptr()) if t is not None else C.c_void_p(0)
+    return t.data_ptr() if t is not None else None
+
+
+@functools.lru_cache(maxsize=1024)
+def _rows_workspace(n, k, score_type, top):
+    return lib.cd_rows_workspace(n, k, score_type, top)
 
 
 SCORE_TYPES = {torch.float32: _lib.CD_T_F32, torch.bfloat16: _lib.CD_T_BF16, torch.float16: _lib.CD_T_F16}
@@ -72,7 +78,7 @@ class Engine:
 
     # ------------------------------------------------------------------ helpers
     def _stream(self):
-        return C.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
+        return torch._C._cuda_getCurrentRawStream(self.device.index)      # torch.cuda.current_stream without its object
 
     def _check_dev(self, t, name, dtype):
         if not torch.is_tensor(t) or t.device != self.device:
@@ -290,7 +296,7 @@ class Engine:
 
     def _workspace(self, scores, top):
         n, k = scores.shape
-        size = lib.cd_rows_workspace(n, k, SCORE_TYPES[scores.dtype], top)
+        size = _rows_workspace(n, k, SCORE_TYPES[scores.dtype], top)
         return torch.empty((size,), dtype=torch.uint8, device=self.device) if size else None, size
 
     def log_probs(self, scores, ids=None, top=0, temperature=1.0, entropy=True):
