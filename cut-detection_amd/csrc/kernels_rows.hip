@@ -33,7 +33,7 @@ typedef u32x4 __attribute__((aligned(2))) u32x4_any;      // 16 bytes at any ele
 
 template <int TYPE> struct Elem;
 template <> struct Elem<CD_T_F32> {
-    static constexpr int kVec = 4, kZeroBits = 0;        // (kZeroBits: low bits of a float that the type leaves 0)
+    static constexpr int kSize = 4, kVec = 4, kZeroBits = 0;        // (kZeroBits: low bits of a float that the type leaves 0)
     static constexpr uint32_t kNegInf = 0xff800000u;
     static __device__ __forceinline__ float load(const char* row, int64_t i) {
         return reinterpret_cast<const float*>(row)[i];
@@ -49,7 +49,7 @@ template <> struct Elem<CD_T_F32> {
     }
 };
 template <> struct Elem<CD_T_BF16> {
-    static constexpr int kVec = 8, kZeroBits = 16;
+    static constexpr int kSize = 2, kVec = 8, kZeroBits = 16;
     static constexpr uint32_t kNegInf = 0xff80ff80u;
     static __device__ __forceinline__ float load(const char* row, int64_t i) {
         return __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(row)[i] << 16);
@@ -70,7 +70,7 @@ template <> struct Elem<CD_T_BF16> {
     }
 };
 template <> struct Elem<CD_T_F16> {
-    static constexpr int kVec = 8, kZeroBits = 13;
+    static constexpr int kSize = 2, kVec = 8, kZeroBits = 13;
     static constexpr uint32_t kNegInf = 0xfc00fc00u;
     static __device__ __forceinline__ float load(const char* row, int64_t i) {
         return (float)reinterpret_cast<const _Float16*>(row)[i];
@@ -205,6 +205,13 @@ __device__ __forceinline__ uint64_t wave_max_key(uint64_t v) {
     return v;
 }
 
+// A row split between `parts` workgroups (grid y): part p has the scores [lo, hi), lo a multiple of 64.
+struct Part { int lo, hi; };
+__device__ __forceinline__ Part part_of(int k, int parts, int p) {
+    const int64_t share = ((int64_t)(k + parts - 1) / parts + 63) / 64 * 64;
+    return {(int)min((int64_t)k, share * p), (int)min((int64_t)k, share * (p + 1))};
+}
+
 struct LogProbsArgs {
     const char* x;
     int64_t n, row_bytes;
@@ -213,6 +220,9 @@ struct LogProbsArgs {
     const int64_t* ids;
     float *stats, *logp, *entropy, *top_logp;
     int64_t* top_ids;
+    int parts;                      // of a row split between workgroups: what they find, [n][parts] and [n][parts][top]
+    float4* part_stats;
+    uint64_t* part_keys;
 };
 
 __device__ __forceinline__ float entropy_of(const Stat& a) {
@@ -255,7 +265,7 @@ __device__ __forceinline__ void write_top(const LogProbsArgs& A, int64_t row, in
 constexpr int kDense = 24;
 template <int THREADS> struct BlockShared {
     static constexpr int kWaves = THREADS / 64, kList = 1024;
-    float m[kWaves], s[kWaves], u[kWaves];
+    float m[kWaves], s[kWaves], u[kWaves], total;
     uint32_t group[64];
     int count, above, dense, part[kWaves];
     uint8_t lane[kWaves][64];
@@ -274,6 +284,27 @@ __device__ __forceinline__ uint32_t kth_key(uint32_t key, int K) {
     }
     t <<= ZERO_BITS;
     return t & 0x80000000u ? t : t | ((1u << ZERO_BITS) - 1u);        // (keys of negative scores end in ones)
+}
+
+// The statistics of all threads' parts, the same bits in every thread; one barrier.
+template <int THREADS>
+__device__ __forceinline__ Stat block_merge(Stat a, float c, BlockShared<THREADS>& sh) {
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    constexpr int G = THREADS / 64;                       // threads of a group
+    float g = a.m;
+    if (G > 1) g = fmaxf(g, dpp<0x111, 0xf>(-kInf, g));
+    if (G > 2) g = fmaxf(g, dpp<0x112, 0xf>(-kInf, g));
+    if (G > 4) g = fmaxf(g, dpp<0x114, 0xf>(-kInf, g));
+    if (G > 8) g = fmaxf(g, dpp<0x118, 0xf>(-kInf, g));
+    if (tid % G == G - 1) sh.group[tid / G] = score_key(g);
+    a = wave_merge(a, c);
+    if (lane == 0) { sh.m[wave] = a.m; sh.s[wave] = a.s; sh.u[wave] = a.u; }
+    if (tid == 0) sh.count = sh.above = sh.dense = 0;
+    __syncthreads();
+    a.m = lane < THREADS / 64 ? sh.m[lane] : -kInf;
+    a.s = lane < THREADS / 64 ? sh.s[lane] : 0.f;
+    a.u = lane < THREADS / 64 ? sh.u[lane] : 0.f;
+    return wave_merge(a, c);
 }
 
 // The pass over a row; `mine` receives the maximum of the calling thread's scores.
@@ -299,22 +330,7 @@ __device__ __forceinline__ Stat block_stat(const char* x, int k, float c, BlockS
         accumulate<1, ENT>(&xt, a, c);
     }
     *mine = a.m;
-    constexpr int G = THREADS / 64;                       // threads of a group
-    float g = a.m;
-    if (G > 1) g = fmaxf(g, dpp<0x111, 0xf>(-kInf, g));
-    if (G > 2) g = fmaxf(g, dpp<0x112, 0xf>(-kInf, g));
-    if (G > 4) g = fmaxf(g, dpp<0x114, 0xf>(-kInf, g));
-    if (G > 8) g = fmaxf(g, dpp<0x118, 0xf>(-kInf, g));
-    if (tid % G == G - 1) sh.group[tid / G] = score_key(g);
-    a = wave_merge(a, c);
-    const int wave = tid >> 6, lane = tid & 63;
-    if (lane == 0) { sh.m[wave] = a.m; sh.s[wave] = a.s; sh.u[wave] = a.u; }
-    if (tid == 0) sh.count = sh.above = sh.dense = 0;
-    __syncthreads();
-    a.m = lane < THREADS / 64 ? sh.m[lane] : -kInf;
-    a.s = lane < THREADS / 64 ? sh.s[lane] : 0.f;
-    a.u = lane < THREADS / 64 ? sh.u[lane] : 0.f;
-    return wave_merge(a, c);
+    return block_merge(a, c, sh);
 }
 
 // Calls emit(rank, key) for the K highest of the k scores, every rank once, by any thread.
@@ -410,6 +426,101 @@ __global__ __launch_bounds__(THREADS) void log_probs_block_kernel(LogProbsArgs A
     }
 }
 
+// Few, long rows: several workgroups per row leave their statistics and highest classes in the workspace, and one wave
+// per row joins them.
+template <int TYPE, int THREADS, bool ENT>
+__global__ __launch_bounds__(THREADS) void log_probs_part_kernel(LogProbsArgs A) {
+    __shared__ BlockShared<THREADS> sh;
+    const int64_t row = blockIdx.x, slot = row * A.parts + blockIdx.y;
+    const Part p = part_of(A.k, A.parts, blockIdx.y);
+    const char* x = A.x + row * A.row_bytes + (int64_t)p.lo * Elem<TYPE>::kSize;
+    float mine;
+    const Stat a = block_stat<TYPE, THREADS, ENT>(x, p.hi - p.lo, A.c, sh, &mine);
+    if (threadIdx.x == 0) A.part_stats[slot] = {a.m, a.s, a.u, 0.f};
+    if (A.top) {
+        uint64_t* keys = A.part_keys + slot * A.top;
+        const int have = min(A.top, p.hi - p.lo);
+        for (int r = have + threadIdx.x; r < A.top; r += THREADS) keys[r] = 0;
+        if (have) block_top<TYPE>(x, p.hi - p.lo, have, mine, a.s != a.s, sh,
+                                  [&](int rank, uint64_t key) { keys[rank] = key - p.lo; });
+    }
+}
+__device__ __forceinline__ Stat join_stats(const float4* part, int parts, float c) {
+    const int lane = threadIdx.x & 63;
+    Stat a = {-kInf, 0.f, 0.f};
+    if (lane < parts) { const float4 v = part[lane]; a = {v.x, v.y, v.z}; }
+    return wave_merge(a, c);
+}
+template <int TYPE>
+__global__ __launch_bounds__(64) void log_probs_join_kernel(LogProbsArgs A) {
+    __shared__ uint64_t list[64 * kMaxTop];
+    const int lane = threadIdx.x;
+    const int64_t row = blockIdx.x;
+    const Stat a = join_stats(A.part_stats + row * A.parts, A.parts, A.c);
+    if (lane == 0) write_row<TYPE>(A, row, A.x + row * A.row_bytes, a);
+    if (!A.top) return;
+    // of every part the first 64 / parts: 64 keys, whose K-th largest is a bound as in block_top
+    const uint64_t* keys = A.part_keys + row * A.parts * A.top;
+    const int heads = 64 / A.parts, q = lane / heads, r = lane - q * heads;
+    const uint64_t mine = q < A.parts && r < A.top ? keys[q * A.top + r] : 0;
+    uint64_t t = 0;
+    for (int b = 63; b >= 0; --b) {
+        const uint64_t up = t | 1ull << b;
+        if (__popcll(__ballot(mine >= up)) >= A.top) t = up;
+    }
+    int count = 0;
+    for (int e = lane; e - lane < A.parts * A.top; e += 64) {
+        const uint64_t key = e < A.parts * A.top ? keys[e] : 0;
+        const bool take = key != 0 && key >= t;
+        const uint64_t taken = __ballot(take);
+        if (take) list[count + __popcll(taken & ((1ull << lane) - 1))] = key;
+        count += __popcll(taken);
+    }
+    __syncthreads();
+    for (int e = lane; e < count; e += 64) {
+        const uint64_t key = list[e];
+        int rank = 0;
+        for (int j = 0; j < count; ++j) rank += list[j] > key;
+        if (rank < A.top) write_top(A, row, rank, key, a);
+    }
+}
+
+// Writes f(score) for every score of a row, backwards: what the pass before has read last is in the caches, and the
+// writes go past them (4096 x 131072 bf16 as the second half of distill: 570 us with ordinary stores, 525 so; forwards
+// 587 and 569).  dx may be x itself.
+template <int TYPE, int THREADS, class F>
+__device__ __forceinline__ void sweep(const char* x, char* dx, int k, F f) {
+    using E = Elem<TYPE>;
+    constexpr int U = 4, VE = E::kVec;
+    const int nv = k / VE, tid = threadIdx.x, last = nv * VE + tid;
+    if (last < k) E::store(dx, last, f(E::load(x, last)));
+    for (int v0 = (nv - 1) / (U * THREADS) * (U * THREADS); v0 >= 0; v0 -= U * THREADS) {
+        u32x4 w[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int v = v0 + u * THREADS + tid;
+            if (v < nv) w[u] = reinterpret_cast<const u32x4_any*>(x)[v];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int v = v0 + u * THREADS + tid;
+            float d[VE];
+            E::unpack(w[u], d);
+#pragma unroll
+            for (int i = 0; i < VE; ++i) d[i] = f(d[i]);
+            if (v < nv) __builtin_nontemporal_store(E::pack(d), reinterpret_cast<u32x4_any*>(dx) + v);
+        }
+    }
+}
+// Zeroes a row.
+template <int TYPE, int THREADS>
+__device__ __forceinline__ void clear(char* dx, int k) {
+    using E = Elem<TYPE>;
+    const int nv = k / E::kVec, tid = threadIdx.x, last = nv * E::kVec + tid;
+    for (int v = tid; v < nv; v += THREADS) __builtin_nontemporal_store(u32x4{0, 0, 0, 0}, reinterpret_cast<u32x4_any*>(dx) + v);
+    if (last < k) E::store(dx, last, 0.f);
+}
+
 // ---- gradients ---------------------------------------------------------------------------------------------------
 // d(g_l ln p_id + g_h entropy) / dx_i = [g_l (i == id) - p_i (g_l + g_h (ln p_i + entropy))] / T
 struct LogProbsGradArgs {
@@ -441,25 +552,21 @@ __device__ __forceinline__ float grad_of(float t, const GradRow& g) {
 
 template <int TYPE, int THREADS>
 __global__ __launch_bounds__(THREADS) void log_probs_grad_kernel(LogProbsGradArgs A) {
-    using E = Elem<TYPE>;
-    for (int64_t row = blockIdx.x; row < A.n; row += gridDim.x) {
-        const char* x = A.x + row * A.row_bytes;
-        char* dx = A.dx + row * A.dx_row_bytes;
+    const Part p = part_of(A.k, gridDim.y, blockIdx.y);
+    for (int64_t back = blockIdx.x; back < A.n; back += gridDim.x) {
+        const int64_t row = A.n - 1 - back;               // the rows that the forward call has read last come first
         const float m = A.stats[2 * row], s = A.stats[2 * row + 1];
         const GradRow g = grad_row(A, row, s);
         const Ref t_of(m, A.c);
-        const int nv = A.k / E::kVec;
-        for (int v = blockIdx.y * THREADS + threadIdx.x; v < nv; v += gridDim.y * THREADS) {
-            float xs[E::kVec], d[E::kVec];
-            E::unpack(reinterpret_cast<const u32x4_any*>(x)[v], xs);
-#pragma unroll
-            for (int i = 0; i < E::kVec; ++i) d[i] = grad_of(t_of(xs[i]), g);
-            if (g.id >= 0 && g.id / E::kVec == v)
-                for (int i = 0; i < E::kVec; ++i) if (g.id % E::kVec == i) d[i] += g.hit;
-            reinterpret_cast<u32x4_any*>(dx)[v] = E::pack(d);
-        }
-        const int i = nv * E::kVec + threadIdx.x;
-        if (blockIdx.y == 0 && i < A.k) E::store(dx, i, grad_of(t_of(E::load(x, i)), g) + (i == g.id ? g.hit : 0.f));
+        const char* x = A.x + row * A.row_bytes + (int64_t)p.lo * Elem<TYPE>::kSize;
+        char* dx = A.dx + row * A.dx_row_bytes + (int64_t)p.lo * Elem<TYPE>::kSize;
+        const bool here = g.id >= p.lo && g.id < p.hi;
+        const float hit = here ? grad_of(t_of(Elem<TYPE>::load(x, g.id - p.lo)), g) + g.hit : 0.f;
+        __syncthreads();                                  // (dx may be x)
+        if (t_of.fast) sweep<TYPE, THREADS>(x, dx, p.hi - p.lo, [&](float v) { return grad_of(__builtin_fmaf(v, A.c, -t_of.mc), g); });
+        else sweep<TYPE, THREADS>(x, dx, p.hi - p.lo, [&](float v) { return grad_of(t_of(v), g); });
+        __syncthreads();                                  // the row first, then its class
+        if (threadIdx.x == 0 && here) Elem<TYPE>::store(dx, g.id - p.lo, hit);
     }
 }
 
@@ -476,35 +583,43 @@ struct DistillArgs {
     const void* teacher;
     const float *weights, *g_loss;  // g_loss: only the gradient, each row's times g_loss
     float *stats, *loss;
+    int parts;                      // of a row split between workgroups: what they find, [n][parts], and the student's
+    float4* part_stats;             // scores of the entries [n][entries]
+    float* part_x;
 };
 template <int PER> struct Teacher { // the entries of one row, spread over a wave: entry lane + 64 e, e < PER
     int id[PER];                    // -1: unused
-    float lq[PER];                  // log2 q
+    float lq[PER];                  // the teacher's score, then log2 q
     float q[PER];
+    float sum[PER];                 // of a class named more than once: its q's together at its first entry, else -1
     float x[PER];                   // the student's score
     float total;                    // sum of 2^(..) before normalising: 0 where no entry counts
 };
-template <int TYPE, int PER>
-__device__ __forceinline__ Teacher<PER> load_teacher(const DistillArgs& A, int64_t row, const char* x) {
-    Teacher<PER> r;
+template <int PER>
+__device__ __forceinline__ void load_entries(Teacher<PER>& r, const DistillArgs& A, int64_t row) {
     const int lane = threadIdx.x & 63;
-    float m = -kInf;
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
         const int j = lane + 64 * e;
         int64_t id = -1;
         float v = -kInf;
-        if (j < A.entries) id = A.ids[row * A.entries + j];
+        if (j < A.entries) {
+            id = A.ids[row * A.entries + j];
+            v = load_any(A.teacher_type, A.teacher, row * A.entries + j);
+        }
         const bool used = id >= 0 && id < A.k;
-        if (used) v = load_any(A.teacher_type, A.teacher, row * A.entries + j);
         r.id[e] = used ? (int)id : -1;
-        r.lq[e] = v;
-        r.x[e] = used ? Elem<TYPE>::load(x, id) : 0.f;
-        m = fmaxf(m, v);
+        r.lq[e] = used ? v : -kInf;
     }
+}
+template <int PER>
+__device__ __forceinline__ void share_out(Teacher<PER>& r, const DistillArgs& A) {
+    const int lane = threadIdx.x & 63;
+    float m = -kInf, total = 0.f;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) m = fmaxf(m, r.lq[e]);
     m = wave_max(m);
     const Ref t_of(m, A.c);
-    float total = 0.f;
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
         r.lq[e] = t_of(r.lq[e]);
@@ -513,9 +628,30 @@ __device__ __forceinline__ Teacher<PER> load_teacher(const DistillArgs& A, int64
     }
     r.total = wave_sum(total);
     const float l = __builtin_amdgcn_logf(r.total), inv = 1.f / r.total;
+    bool first[PER];
 #pragma unroll
-    for (int e = 0; e < PER; ++e) { r.lq[e] -= l; r.q[e] *= inv; }
-    return r;
+    for (int e = 0; e < PER; ++e) { r.lq[e] -= l; r.q[e] *= inv; r.sum[e] = 0.f; first[e] = r.id[e] >= 0; }
+    if (A.dx) {
+#pragma unroll
+        for (int f = 0; f < PER; ++f)
+            for (int l = 0; l < min(64, A.entries - 64 * f); ++l) {
+                const int id = __builtin_amdgcn_readlane(r.id[f], l);
+                const float q = lane_of(r.q[f], l);
+#pragma unroll
+                for (int e = 0; e < PER; ++e)
+                    if (id == r.id[e]) {
+                        r.sum[e] += q;
+                        if (64 * f + l < 64 * e + lane) first[e] = false;
+                    }
+            }
+#pragma unroll
+        for (int e = 0; e < PER; ++e) if (!first[e]) r.sum[e] = -1.f;
+    }
+}
+template <int TYPE, int PER>
+__device__ __forceinline__ void load_student(Teacher<PER>& r, const char* x, Part p) {
+#pragma unroll
+    for (int e = 0; e < PER; ++e) r.x[e] = r.id[e] >= p.lo && r.id[e] < p.hi ? Elem<TYPE>::load(x, r.id[e]) : 0.f;
 }
 // one entry's part of a loss of weight and temperature 1
 __device__ __forceinline__ float loss_term(float q, float lq, float x, const Stat& a, float c, float temperature) {
@@ -530,115 +666,192 @@ __device__ __forceinline__ float teacher_loss(const Teacher<PER>& r, const Stat&
         if (r.id[e] >= 0) sum += loss_term(r.q[e], r.lq[e], r.x[e], a, A.c, A.t);
     return w * (A.t * A.t) * wave_sum(sum);
 }
-// gradient at the teacher's classes: of a class named twice the first entry has the sum, the others none
+// the gradient at the teacher's classes, over what the sweep has written there
 template <int TYPE, int PER>
-__device__ __forceinline__ void fix_gradient(const Teacher<PER>& r, const Stat& a, const DistillArgs& A, float w, char* dx) {
+__device__ __forceinline__ void fix_gradient(const Teacher<PER>& r, const Stat& a, const DistillArgs& A, float w, char* dx,
+                                             Part p) {
     const Ref t_of(a.m, A.c);
     const float inv = 1.f / a.s;
-    const int lane = threadIdx.x & 63;
-    float sum[PER];
-    bool first[PER];
-#pragma unroll
-    for (int e = 0; e < PER; ++e) { sum[e] = 0.f; first[e] = r.id[e] >= 0; }
-#pragma unroll
-    for (int f = 0; f < PER; ++f)
-        for (int l = 0; l < min(64, A.entries - 64 * f); ++l) {
-            const int id = __builtin_amdgcn_readlane(r.id[f], l);
-            const float q = lane_of(r.q[f], l);
-#pragma unroll
-            for (int e = 0; e < PER; ++e)
-                if (id == r.id[e]) {
-                    sum[e] += q;
-                    if (64 * f + l < 64 * e + lane) first[e] = false;
-                }
-        }
 #pragma unroll
     for (int e = 0; e < PER; ++e)
-        if (first[e]) Elem<TYPE>::store(dx, r.id[e], w * A.t * (__builtin_amdgcn_exp2f(t_of(r.x[e])) * inv - sum[e]));
+        if (!(r.sum[e] < 0.f) && r.id[e] >= p.lo && r.id[e] < p.hi)
+            Elem<TYPE>::store(dx, r.id[e], w * A.t * (__builtin_amdgcn_exp2f(t_of(r.x[e])) * inv - r.sum[e]));
+}
+
+// w T p of every class of a part
+template <int TYPE, int THREADS>
+__device__ __forceinline__ void distill_sweep(const DistillArgs& A, int64_t row, Part p, const Stat& a, float w) {
+    const char* x = A.x + row * A.row_bytes + (int64_t)p.lo * Elem<TYPE>::kSize;
+    char* dx = A.dx + row * A.dx_row_bytes + (int64_t)p.lo * Elem<TYPE>::kSize;
+    const Ref t_of(a.m, A.c);
+    const float f = w * A.t / a.s;
+    if (t_of.fast)
+        sweep<TYPE, THREADS>(x, dx, p.hi - p.lo, [&](float v) { return f * __builtin_amdgcn_exp2f(__builtin_fmaf(v, A.c, -t_of.mc)); });
+    else
+        sweep<TYPE, THREADS>(x, dx, p.hi - p.lo, [&](float v) { return f * __builtin_amdgcn_exp2f(t_of(v)); });
+}
+
+// What the kernels below share: the row's weight, its teacher (wave 0; every thread learns whether an entry counts), its
+// statistics from `pass`, the loss (part 0), and the gradient of part p from `grad(w, a)`, which writes w T p of every
+// class.  `student` loads the student's scores of the teacher's classes.
+template <int TYPE, int THREADS, int PER, class Student, class Pass, class Grad>
+__device__ __forceinline__ void distill_row(const DistillArgs& A, int64_t row, Part p, BlockShared<THREADS>& sh,
+                                            Student student, Pass pass, Grad grad) {
+    char* dx = A.dx + row * A.dx_row_bytes;
+    const int tid = threadIdx.x;
+    float w = A.weights ? A.weights[row] : 1.f;
+    if (A.g_loss && w != 0.f) w *= A.g_loss[row];
+    Stat a = {-kInf, 0.f, 0.f};
+    Teacher<PER> te;
+    bool on = false;
+    if (w != 0.f) {
+        if (tid < 64) {
+            load_entries<PER>(te, A, row);
+            share_out<PER>(te, A);
+            student(te);
+            if (tid == 0) sh.total = te.total;
+        }
+        a = pass();                                       // (has a barrier: all of x has been read that is read here)
+        on = sh.total != 0.f;
+    }
+    if (A.loss && p.lo == 0 && tid < 64) {
+        const float loss = on ? teacher_loss<PER>(te, a, A, w) : 0.f;
+        if (tid == 0) {
+            A.loss[row] = loss;
+            A.stats[2 * row] = a.m;
+            A.stats[2 * row + 1] = a.s;
+        }
+    }
+    if (A.dx) {
+        const bool live = on && a.s != 0.f;
+        if (live) grad(w, a);
+        else clear<TYPE, THREADS>(dx + (int64_t)p.lo * Elem<TYPE>::kSize, p.hi - p.lo);
+        __syncthreads();                                  // the row first, then the teacher's classes
+        if (live && tid < 64) fix_gradient<TYPE, PER>(te, a, A, w, dx, p);
+    }
+    __syncthreads();
 }
 
 template <int TYPE, int THREADS, int PER>
 __global__ __launch_bounds__(THREADS) void distill_block_kernel(DistillArgs A) {
-    using E = Elem<TYPE>;
     __shared__ BlockShared<THREADS> sh;
-    const int tid = threadIdx.x;
+    const Part all = {0, A.k};
     for (int64_t row = blockIdx.x; row < A.n; row += gridDim.x) {
         const char* x = A.x + row * A.row_bytes;
-        char* dx = A.dx + row * A.dx_row_bytes;
-        const float w = A.weights ? A.weights[row] : 1.f;
-        Stat a = {-kInf, 0.f, 0.f};
-        Teacher<PER> te;
-        te.total = 0.f;
-        if (w != 0.f) {
-            te = load_teacher<TYPE, PER>(A, row, x);           // (every wave: the total decides for all of them)
-            float mine;
-            a = block_stat<TYPE, THREADS, false>(x, A.k, A.c, sh, &mine);
-        }
-        const bool on = w != 0.f && te.total != 0.f;
-        if (tid < 64) {
-            const float loss = on ? teacher_loss(te, a, A, w) : 0.f;
-            if (tid == 0) {
-                A.loss[row] = loss;
-                A.stats[2 * row] = a.m;
-                A.stats[2 * row + 1] = a.s;
-            }
-        }
-        if (A.dx) {
-            const Ref t_of(a.m, A.c);
-            const bool live = on && a.s != 0.f;
-            const float f = live ? w * A.t / a.s : 0.f;
-            const int nv = A.k / E::kVec;
-            for (int v = tid; v < nv; v += THREADS) {
-                float d[E::kVec] = {};
-                if (live) {
-                    E::unpack(reinterpret_cast<const u32x4_any*>(x)[v], d);
-#pragma unroll
-                    for (int i = 0; i < E::kVec; ++i) d[i] = f * __builtin_amdgcn_exp2f(t_of(d[i]));
-                }
-                reinterpret_cast<u32x4_any*>(dx)[v] = E::pack(d);
-            }
-            const int i = nv * E::kVec + tid;
-            if (i < A.k) E::store(dx, i, live ? f * __builtin_amdgcn_exp2f(t_of(E::load(x, i))) : 0.f);
-            __syncthreads();
-            if (live && tid < 64) fix_gradient<TYPE, PER>(te, a, A, w, dx);
-        }
-        __syncthreads();
+        float mine;
+        distill_row<TYPE, THREADS, PER>(A, row, all, sh,
+            [&](Teacher<PER>& te) { load_student<TYPE, PER>(te, x, all); },
+            [&] { return block_stat<TYPE, THREADS, false>(x, A.k, A.c, sh, &mine); },
+            [&](float w, const Stat& a) { distill_sweep<TYPE, THREADS>(A, row, all, a, w); });
     }
 }
 
-// the gradient alone, for a loss gradient g per row, from the statistics of the forward call
+// Few, long rows, as in log_probs: the parts' statistics first, then loss and gradient, part by part again.
+template <int TYPE, int THREADS>
+__global__ __launch_bounds__(THREADS) void distill_part_kernel(DistillArgs A) {
+    __shared__ BlockShared<THREADS> sh;
+    const int64_t row = blockIdx.x;
+    if (A.weights && A.weights[row] == 0.f) return;
+    const Part p = part_of(A.k, A.parts, blockIdx.y);
+    const char* x = A.x + row * A.row_bytes;
+    const int j = threadIdx.x;
+    if (blockIdx.y == 0 && j < A.entries) {               // before the gradient, which may take the scores' place
+        const int64_t id = A.ids[row * A.entries + j];
+        A.part_x[row * A.entries + j] = id >= 0 && id < A.k ? Elem<TYPE>::load(x, id) : 0.f;
+    }
+    float mine;
+    const Stat a = block_stat<TYPE, THREADS, false>(x + (int64_t)p.lo * Elem<TYPE>::kSize, p.hi - p.lo, A.c, sh, &mine);
+    if (threadIdx.x == 0) A.part_stats[row * A.parts + blockIdx.y] = {a.m, a.s, 0.f, 0.f};
+}
 template <int TYPE, int THREADS, int PER>
-__global__ __launch_bounds__(THREADS) void distill_grad_kernel(DistillArgs A) {
+__global__ __launch_bounds__(THREADS) void distill_join_kernel(DistillArgs A) {
+    __shared__ BlockShared<THREADS> sh;
+    const int64_t row = blockIdx.x;
+    const Part p = part_of(A.k, gridDim.y, blockIdx.y);   // (grid y is 1 where there is no gradient)
+    distill_row<TYPE, THREADS, PER>(A, row, p, sh,
+        [&](Teacher<PER>& te) {
+#pragma unroll
+            for (int e = 0; e < PER; ++e) {
+                const int j = (threadIdx.x & 63) + 64 * e;
+                te.x[e] = j < A.entries ? A.part_x[row * A.entries + j] : 0.f;
+            }
+        },
+        [&] {
+            __syncthreads();
+            return join_stats(A.part_stats + row * A.parts, A.parts, A.c);
+        },
+        [&](float w, const Stat& a) { distill_sweep<TYPE, THREADS>(A, row, p, a, w); });
+}
+
+// Loss and gradient of rows that fit the threads' registers, V vectors each: they are read once, all loads at once, and
+// the second half of the work starts from the registers.
+template <int TYPE, int THREADS, int V, int PER>
+__global__ __launch_bounds__(THREADS) void distill_held_kernel(DistillArgs A) {
     using E = Elem<TYPE>;
-    const int tid = threadIdx.x;
+    constexpr int VE = E::kVec, U = 2;
+    __shared__ BlockShared<THREADS> sh;
+    const int nv = A.k / VE, tid = threadIdx.x, last = nv * VE + tid;
+    const Part all = {0, A.k};
     for (int64_t row = blockIdx.x; row < A.n; row += gridDim.x) {
         const char* x = A.x + row * A.row_bytes;
         char* dx = A.dx + row * A.dx_row_bytes;
-        const float w = (A.weights ? A.weights[row] : 1.f);
-        const float wg = w == 0.f ? 0.f : w * A.g_loss[row];
-        const Stat a = {A.stats[2 * row], A.stats[2 * row + 1], 0.f};
-        Teacher<PER> te;
-        te.total = 0.f;
-        if (wg != 0.f) te = load_teacher<TYPE, PER>(A, row, x);
-        __syncthreads();                                  // dx may be x: the teacher's classes are read before any write
-        const bool live = wg != 0.f && te.total != 0.f && a.s != 0.f;
-        const Ref t_of(a.m, A.c);
-        const float f = live ? wg * A.t / a.s : 0.f;
-        const int nv = A.k / E::kVec;
-        for (int v = tid; v < nv; v += THREADS) {
-            float d[E::kVec] = {};
-            if (live) {
-                E::unpack(reinterpret_cast<const u32x4_any*>(x)[v], d);
+        u32x4 w[V];
+        float tail = -kInf;
+        distill_row<TYPE, THREADS, PER>(A, row, all, sh,
+            [&](Teacher<PER>& te) { load_student<TYPE, PER>(te, x, all); },
+            [&] {
 #pragma unroll
-                for (int i = 0; i < E::kVec; ++i) d[i] = f * __builtin_amdgcn_exp2f(t_of(d[i]));
-            }
-            reinterpret_cast<u32x4_any*>(dx)[v] = E::pack(d);
-        }
-        const int i = nv * E::kVec + tid;
-        if (i < A.k) E::store(dx, i, live ? f * __builtin_amdgcn_exp2f(t_of(E::load(x, i))) : 0.f);
-        __syncthreads();
-        if (live && tid < 64) fix_gradient<TYPE, PER>(te, a, A, wg, dx);
-        __syncthreads();
+                for (int u = 0; u < V; ++u) {
+                    w[u] = u32x4{E::kNegInf, E::kNegInf, E::kNegInf, E::kNegInf};
+                    if (u * THREADS + tid < nv) w[u] = reinterpret_cast<const u32x4_any*>(x + 16 * u * THREADS)[tid];
+                }
+                if (last < A.k) tail = E::load(x, last);
+                Stat a = {-kInf, 0.f, 0.f};
+#pragma unroll
+                for (int u = 0; u < V; u += U) {
+                    float xs[U * VE];
+#pragma unroll
+                    for (int i = 0; i < U; ++i) E::unpack(w[u + i], xs + i * VE);
+                    accumulate<U * VE, false>(xs, a, A.c);
+                }
+                accumulate<1, false>(&tail, a, A.c);
+                return block_merge(a, A.c, sh);
+            },
+            [&](float weight, const Stat& a) {
+                const Ref t_of(a.m, A.c);
+                const float f = weight * A.t / a.s;
+#pragma unroll
+                for (int u = 0; u < V; ++u) {
+                    float d[VE];
+                    E::unpack(w[u], d);
+                    if (t_of.fast) {
+#pragma unroll
+                        for (int i = 0; i < VE; ++i) d[i] = f * __builtin_amdgcn_exp2f(__builtin_fmaf(d[i], A.c, -t_of.mc));
+                    } else {
+                        for (int i = 0; i < VE; ++i) d[i] = f * __builtin_amdgcn_exp2f(t_of(d[i]));
+                    }
+                    if (u * THREADS + tid < nv)
+                        __builtin_nontemporal_store(E::pack(d), reinterpret_cast<u32x4_any*>(dx + 16 * u * THREADS) + tid);
+                }
+                if (last < A.k) E::store(dx, last, f * __builtin_amdgcn_exp2f(t_of(tail)));
+            });
+    }
+}
+
+// the gradient alone, from the statistics of the forward call
+template <int TYPE, int THREADS, int PER>
+__global__ __launch_bounds__(THREADS) void distill_grad_kernel(DistillArgs A) {
+    __shared__ BlockShared<THREADS> sh;
+    const Part p = part_of(A.k, gridDim.y, blockIdx.y);
+    for (int64_t back = blockIdx.x; back < A.n; back += gridDim.x) {
+        const int64_t row = A.n - 1 - back;
+        distill_row<TYPE, THREADS, PER>(A, row, p, sh,
+            [&](Teacher<PER>& te) { load_student<TYPE, PER>(te, A.x + row * A.row_bytes, p); },
+            [&] {
+                __syncthreads();
+                return Stat{A.stats[2 * row], A.stats[2 * row + 1], 0.f};
+            },
+            [&](float w, const Stat& a) { distill_sweep<TYPE, THREADS>(A, row, p, a, w); });
     }
 }
 
@@ -854,7 +1067,9 @@ __global__ __launch_bounds__(256) void distill_wave_kernel(DistillArgs A) {
         te.total = 0.f;
         if (w != 0.f) {
             load_spread<TYPE, N>(x, A.k, v);
-            te = load_teacher<TYPE, PER>(A, row, x);
+            load_entries<PER>(te, A, row);
+            share_out<PER>(te, A);
+            load_student<TYPE, PER>(te, x, Part{0, A.k});
             accumulate<N, false>(v, a, A.c);
             a = wave_merge(a, A.c);
         }
@@ -875,7 +1090,7 @@ __global__ __launch_bounds__(256) void distill_wave_kernel(DistillArgs A) {
                 if (lane + 64 * j < A.k)
                     Elem<TYPE>::store(dx, lane + 64 * j, live ? f * __builtin_amdgcn_exp2f(t_of(v[j])) : 0.f);
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");      // the row first, then the teacher's classes
-            if (live) fix_gradient<TYPE, PER>(te, a, A, w, dx);
+            if (live) fix_gradient<TYPE, PER>(te, a, A, w, dx, Part{0, A.k});
         }
     }
 }
@@ -883,11 +1098,16 @@ __global__ __launch_bounds__(256) void distill_wave_kernel(DistillArgs A) {
 constexpr int64_t kMaxGrid = 1 << 20;       // workgroups of a launch; further rows are taken by a loop
 unsigned row_grid(int64_t n) { return (unsigned)std::min(n, kMaxGrid); }
 
+// Threads of a workgroup that reads a row of more than kWaveClasses scores: many for few rows, since a row's time is then
+// what counts; else as few as keep a few pieces of 64 bytes per thread, so that several rows share a CU and one's reads
+// fill another's waits (4096 rows, 20 alternatives: 8000 x bf16 27 us with 256 threads, 42 with 512, 111 with 1024; 128000 x
+// bf16 263, 217 and 249; 64 rows of 131072 x bf16: 29, 19 and 16).
 int block_threads(const RowsIn& in) {
 #ifdef CD_EXP_ENV
     if (const char* e = std::getenv("CUTDET_X_THREADS")) return std::atoi(e);
 #endif
-    return in.k > 32768 ? 1024 : 256;
+    const int64_t bytes = (int64_t)in.k * (in.type == CD_T_F32 ? 4 : 2);
+    return bytes <= 32768 ? 256 : in.n <= 256 && bytes > 65536 ? 1024 : 512;
 }
 
 // CALL(type, ...) for the type of the scores
@@ -901,15 +1121,37 @@ int block_threads(const RowsIn& in) {
 unsigned thread_grid(int64_t n) { return row_grid((n + 63) / 64); }
 unsigned wave_grid(int64_t n) { return row_grid((n + 3) / 4); }
 int elem_size(int type) { return type == CD_T_F32 ? 4 : 2; }
+constexpr int64_t kSplitBytes = 128 << 10, kSplitRows = 64;
 
 }  // namespace
 
-size_t rows_workspace(int64_t n, int k, int type, int top) { return 0; }
+// Workgroups per row of the calls that need a second kernel to join them.
+static int join_parts(int64_t n, int k, int type) {
+    const int64_t bytes = (int64_t)k * elem_size(type);
+    if (bytes < kSplitBytes || n > kSplitRows) return 1;
+    int parts = 2;
+    while (parts < 64 && n * parts < 512 && bytes / parts > 32768) parts *= 2;
+    return parts;
+}
+// ... and of the gradients, whose parts need no join
+static unsigned grad_parts(int64_t n, int k, int type) {
+    const int64_t bytes = (int64_t)k * elem_size(type);
+    return (unsigned)std::max<int64_t>(1, std::min<int64_t>(1024 / n, bytes / 16384));
+}
+
+size_t rows_workspace(int64_t n, int k, int type, int top) {
+    const int parts = join_parts(n, k, type);
+    return parts == 1 ? 0 : (size_t)n * (parts * (sizeof(float4) + top * sizeof(uint64_t)) + kMaxTeacher * sizeof(float));
+}
 
 int launch_log_probs(const RowsIn& in, const int64_t* ids, int top, float* stats, float* logp, float* entropy,
                      float* top_logp, int64_t* top_ids, void* workspace, hipStream_t s) {
-    const LogProbsArgs A = {static_cast<const char*>(in.x), in.n, in.stride * elem_size(in.type), in.k, top,
-                            kLog2e / in.temperature, in.temperature, ids, stats, logp, entropy, top_logp, top_ids};
+    LogProbsArgs A = {static_cast<const char*>(in.x), in.n, in.stride * elem_size(in.type), in.k, top,
+                      kLog2e / in.temperature, in.temperature, ids, stats, logp, entropy, top_logp, top_ids};
+    A.parts = join_parts(in.n, in.k, in.type);
+    A.part_stats = static_cast<float4*>(workspace);
+    A.part_keys = reinterpret_cast<uint64_t*>(A.part_stats + in.n * A.parts);
+    const dim3 parts((unsigned)in.n, (unsigned)A.parts);
 #define SHORT(TY, K) log_probs_thread_kernel<TY, K><<<thread_grid(in.n), 64, 0, s>>>(A)
 #define WAVE(TY, N)                                                                         \
     if (entropy) log_probs_wave_kernel<TY, N, true><<<wave_grid(in.n), 256, 0, s>>>(A);     \
@@ -917,15 +1159,22 @@ int launch_log_probs(const RowsIn& in, const int64_t* ids, int top, float* stats
 #define BLOCK(TY, TH)                                                                       \
     if (entropy) log_probs_block_kernel<TY, TH, true><<<row_grid(in.n), TH, 0, s>>>(A);     \
     else log_probs_block_kernel<TY, TH, false><<<row_grid(in.n), TH, 0, s>>>(A)
+#define PARTS(TY, TH)                                                                       \
+    if (entropy) log_probs_part_kernel<TY, TH, true><<<parts, TH, 0, s>>>(A);               \
+    else log_probs_part_kernel<TY, TH, false><<<parts, TH, 0, s>>>(A);                      \
+    log_probs_join_kernel<TY><<<(unsigned)in.n, 64, 0, s>>>(A)
     if (in.k <= 4) CD_BY_TYPE(in.type, SHORT, 4);
     else if (in.k <= kThreadClasses) CD_BY_TYPE(in.type, SHORT, kThreadClasses);
     else if (in.k <= 256) CD_BY_TYPE(in.type, WAVE, 4);
     else if (in.k <= kWaveClasses) CD_BY_TYPE(in.type, WAVE, 16);
+    else if (A.parts > 1) CD_BY_TYPE(in.type, PARTS, 512);
     else if (block_threads(in) == 256) CD_BY_TYPE(in.type, BLOCK, 256);
+    else if (block_threads(in) == 512) CD_BY_TYPE(in.type, BLOCK, 512);
     else CD_BY_TYPE(in.type, BLOCK, 1024);
 #undef SHORT
 #undef WAVE
 #undef BLOCK
+#undef PARTS
     CD_HIP(hipGetLastError());
     return CD_OK;
 }
@@ -938,7 +1187,8 @@ int launch_log_probs_backward(const RowsIn& in, const int64_t* ids, const float*
                                 entropy, g_logp, g_entropy};
 #define SHORT(TY, K) log_probs_grad_thread_kernel<TY, K><<<thread_grid(in.n), 64, 0, s>>>(A)
 #define WAVE(TY, N) log_probs_grad_wave_kernel<TY, N><<<wave_grid(in.n), 256, 0, s>>>(A)
-#define BLOCK(TY, TH) log_probs_grad_kernel<TY, TH><<<row_grid(in.n), TH, 0, s>>>(A)
+    const dim3 grid(row_grid(in.n), grad_parts(in.n, in.k, in.type));
+#define BLOCK(TY, TH) log_probs_grad_kernel<TY, TH><<<grid, TH, 0, s>>>(A)
     if (in.k <= 4) CD_BY_TYPE(in.type, SHORT, 4);
     else if (in.k <= kThreadClasses) CD_BY_TYPE(in.type, SHORT, kThreadClasses);
     else if (in.k <= 256) CD_BY_TYPE(in.type, WAVE, 4);
@@ -977,14 +1227,34 @@ static bool launch_short_distill(const RowsIn& in, const DistillArgs& A, hipStre
 
 int launch_distill(const RowsIn& in, const TeacherIn& te, float* stats, float* loss, void* dx, int64_t dx_stride,
                    void* workspace, hipStream_t s) {
-    const DistillArgs A = distill_args(in, te, stats, loss, nullptr, dx, dx_stride);
+    DistillArgs A = distill_args(in, te, stats, loss, nullptr, dx, dx_stride);
+    A.parts = join_parts(in.n, in.k, in.type);
+    A.part_stats = static_cast<float4*>(workspace);
+    A.part_x = reinterpret_cast<float*>(A.part_stats + in.n * A.parts);
+    const dim3 parts((unsigned)in.n, (unsigned)A.parts), writers((unsigned)in.n, dx ? grad_parts(in.n, in.k, in.type) : 1);
     if (!launch_short_distill(in, A, s)) {
+#define PARTS(TY, TH)                                                                                       \
+    distill_part_kernel<TY, TH><<<parts, TH, 0, s>>>(A);                                                    \
+    if (A.entries <= 64) distill_join_kernel<TY, 256, 1><<<writers, 256, 0, s>>>(A);                        \
+    else distill_join_kernel<TY, 256, kMaxTeacher / 64><<<writers, 256, 0, s>>>(A)
 #define BLOCK(TY, TH)                                                                                       \
     if (A.entries <= 64) distill_block_kernel<TY, TH, 1><<<row_grid(in.n), TH, 0, s>>>(A);                  \
     else distill_block_kernel<TY, TH, kMaxTeacher / 64><<<row_grid(in.n), TH, 0, s>>>(A)
-        if (block_threads(in) == 256) CD_BY_TYPE(in.type, BLOCK, 256);
+#define HELD(TY, TH, V)                                                                                     \
+    if (A.entries <= 64) distill_held_kernel<TY, TH, V, 1><<<row_grid(in.n), TH, 0, s>>>(A);                \
+    else distill_held_kernel<TY, TH, V, kMaxTeacher / 64><<<row_grid(in.n), TH, 0, s>>>(A)
+        const int vectors = in.k / (16 / elem_size(in.type));
+        if (A.parts > 1) CD_BY_TYPE(in.type, PARTS, 512);
+        else if (vectors <= 256 * 8) CD_BY_TYPE(in.type, HELD, 256, 8);
+        else if (vectors <= 512 * 8) CD_BY_TYPE(in.type, HELD, 512, 8);
+        else if (vectors <= 512 * 16) CD_BY_TYPE(in.type, HELD, 512, 16);
+        else if (vectors <= 1024 * 16) CD_BY_TYPE(in.type, HELD, 1024, 16);
+        else if (block_threads(in) == 256) CD_BY_TYPE(in.type, BLOCK, 256);
+        else if (block_threads(in) == 512) CD_BY_TYPE(in.type, BLOCK, 512);
         else CD_BY_TYPE(in.type, BLOCK, 1024);
 #undef BLOCK
+#undef HELD
+#undef PARTS
     }
     CD_HIP(hipGetLastError());
     return CD_OK;
@@ -995,9 +1265,10 @@ int launch_distill_backward(const RowsIn& in, const TeacherIn& te, const float* 
     DistillArgs A = distill_args(in, te, nullptr, nullptr, g_loss, dx, dx_stride);
     if (!launch_short_distill(in, A, s)) {
         A.stats = const_cast<float*>(stats);              // only read
+        const dim3 grid(row_grid(in.n), grad_parts(in.n, in.k, in.type));
 #define BLOCK(TY, TH)                                                                                       \
-    if (A.entries <= 64) distill_grad_kernel<TY, TH, 1><<<row_grid(in.n), TH, 0, s>>>(A);                   \
-    else distill_grad_kernel<TY, TH, kMaxTeacher / 64><<<row_grid(in.n), TH, 0, s>>>(A)
+    if (A.entries <= 64) distill_grad_kernel<TY, TH, 1><<<grid, TH, 0, s>>>(A);                             \
+    else distill_grad_kernel<TY, TH, kMaxTeacher / 64><<<grid, TH, 0, s>>>(A)
         CD_BY_TYPE(in.type, BLOCK, 256);
 #undef BLOCK
     }
