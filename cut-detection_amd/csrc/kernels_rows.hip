@@ -212,6 +212,26 @@ __device__ __forceinline__ Part part_of(int k, int parts, int p) {
     return {(int)min((int64_t)k, share * p), (int)min((int64_t)k, share * (p + 1))};
 }
 
+// How a workgroup takes a row apart: `head` scores up to a 128-byte border (of the memory that counts most: the one
+// written to, else the one read), vectors of 16 bytes, and the rest.  Thread j < extra has one score of head or rest.  Rows
+// that begin anywhere cost 20 % more to read where the 16 bytes are not on a 4-byte border, and 15 to 20 % more to write
+// where a wave's KB does not cover whole lines (2048 x 130001 bf16: 130 us against 107, gradient 293 against 242).
+template <int TYPE> struct Grid {
+    int head, nv, extra;
+    __device__ __forceinline__ Grid(const char* border, int k) {
+        head = min(k, (int)(-reinterpret_cast<uintptr_t>(border) & 127) / Elem<TYPE>::kSize);
+        nv = (k - head) / Elem<TYPE>::kVec;
+        extra = k - nv * Elem<TYPE>::kVec;
+    }
+    __device__ __forceinline__ int single(int j) const { return j < head ? j : j + nv * Elem<TYPE>::kVec; }
+    __device__ __forceinline__ const u32x4_any* vectors(const char* x) const {
+        return reinterpret_cast<const u32x4_any*>(x + head * Elem<TYPE>::kSize);
+    }
+    __device__ __forceinline__ u32x4_any* vectors(char* x) const {
+        return reinterpret_cast<u32x4_any*>(x + head * Elem<TYPE>::kSize);
+    }
+};
+
 struct LogProbsArgs {
     const char* x;
     int64_t n, row_bytes;
@@ -239,15 +259,16 @@ __device__ __forceinline__ float logp_of(float x, const Stat& a, float c, float 
     return lp > 0.f ? 0.f : lp;
 }
 
-template <int TYPE>
-__device__ __forceinline__ void write_row(const LogProbsArgs& A, int64_t row, const char* x, const Stat& a) {
+// the row's class id, -1 where it is skipped
+__device__ __forceinline__ int id_of(const LogProbsArgs& A, int64_t row) {
+    const int64_t id = A.ids ? A.ids[row] : -1;
+    return id >= 0 && id < A.k ? (int)id : -1;
+}
+__device__ __forceinline__ void write_row(const LogProbsArgs& A, int64_t row, int id, float xid, const Stat& a) {
     A.stats[2 * row] = a.m;
     A.stats[2 * row + 1] = a.s;
     if (A.entropy) A.entropy[row] = entropy_of(a);
-    if (A.logp) {
-        const int64_t id = A.ids[row];
-        A.logp[row] = id >= 0 && id < A.k ? logp_of(Elem<TYPE>::load(x, id), a, A.c, A.t) : 0.f;
-    }
+    if (A.logp) A.logp[row] = id >= 0 ? logp_of(xid, a, A.c, A.t) : 0.f;
 }
 __device__ __forceinline__ void write_top(const LogProbsArgs& A, int64_t row, int rank, uint64_t key, const Stat& a) {
     A.top_ids[row * A.top + rank] = (uint32_t)~(uint32_t)key;
@@ -278,9 +299,13 @@ template <int ZERO_BITS>
 __device__ __forceinline__ uint32_t kth_key(uint32_t key, int K) {
     uint32_t t = 0;
     const uint32_t part = key >> ZERO_BITS;
-    for (int b = 31 - ZERO_BITS; b >= 0; --b) {
-        const uint32_t up = t | 1u << b;
-        if (__popcll(__ballot(part >= up)) >= K) t = up;
+    constexpr int kBits = 32 - ZERO_BITS;
+    if (kBits & 1 && __popcll(__ballot(part >> (kBits - 1) != 0)) >= K) t = 1u << (kBits - 1);
+#pragma unroll
+    for (int b = kBits / 2 * 2 - 2; b >= 0; b -= 2) {     // two bits a step: three counts that do not wait for one another
+        const int c1 = __popcll(__ballot(part >= (t | 1u << b))), c2 = __popcll(__ballot(part >= (t | 2u << b))),
+                  c3 = __popcll(__ballot(part >= (t | 3u << b)));
+        t |= (c3 >= K ? 3u : c2 >= K ? 2u : c1 >= K ? 1u : 0u) << b;
     }
     t <<= ZERO_BITS;
     return t & 0x80000000u ? t : t | ((1u << ZERO_BITS) - 1u);        // (keys of negative scores end in ones)
@@ -307,30 +332,30 @@ __device__ __forceinline__ Stat block_merge(Stat a, float c, BlockShared<THREADS
     return wave_merge(a, c);
 }
 
-// The pass over a row; `mine` receives the maximum of the calling thread's scores.
+// The calling thread's part of the pass over a row.
 template <int TYPE, int THREADS, bool ENT>
-__device__ __forceinline__ Stat block_stat(const char* x, int k, float c, BlockShared<THREADS>& sh, float* mine) {
+__device__ __forceinline__ Stat block_pass(const char* x, int k, float c) {
     using E = Elem<TYPE>;
-    constexpr int U = 4, VE = E::kVec;
-    const int nv = k / VE, tid = threadIdx.x;
+    constexpr int VE = E::kVec, U = 4;
+    const Grid<TYPE> g(x, k);
+    const int tid = threadIdx.x;
+    const u32x4_any* vec = g.vectors(x);
     Stat a = {-kInf, 0.f, 0.f};
-    for (int v0 = 0; v0 < nv; v0 += U * THREADS) {
+    for (int v0 = 0; v0 < g.nv; v0 += U * THREADS) {
         float xs[U * VE];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int v = v0 + u * THREADS + tid;
             u32x4 w = {E::kNegInf, E::kNegInf, E::kNegInf, E::kNegInf};
-            if (v < nv) w = reinterpret_cast<const u32x4_any*>(x)[v];
+            if (v0 + u * THREADS + tid < g.nv) w = vec[v0 + u * THREADS + tid];
             E::unpack(w, xs + u * VE);
         }
         accumulate<U * VE, ENT>(xs, a, c);
     }
-    if (nv * VE + tid < k) {
-        const float xt = E::load(x, nv * VE + tid);
+    if (tid < g.extra) {
+        const float xt = E::load(x, g.single(tid));
         accumulate<1, ENT>(&xt, a, c);
     }
-    *mine = a.m;
-    return block_merge(a, c, sh);
+    return a;
 }
 
 // Calls emit(rank, key) for the K highest of the k scores, every rank once, by any thread.
@@ -338,7 +363,8 @@ template <int TYPE, int THREADS, class Emit>
 __device__ __forceinline__ void block_top(const char* x, int k, int K, float mine, bool nan, BlockShared<THREADS>& sh,
                                           Emit emit) {
     using E = Elem<TYPE>;
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, nv = k / E::kVec;
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    const Grid<TYPE> g(x, k);
     const uint32_t T = kth_key<E::kZeroBits>(sh.group[lane], K);
     if (!nan) {
         const float xt = key_score(T);
@@ -354,18 +380,17 @@ __device__ __forceinline__ void block_top(const char* x, int k, int K, float min
         if (dense && lane == 0) sh.dense = 1;
         if (who >> lane & 1) sh.lane[wave][__popcll(who & ((1ull << lane) - 1))] = lane;
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        const int share = (nv + THREADS - 1) / THREADS, items = __popcll(who) * share;
+        const int share = (g.nv + THREADS - 1) / THREADS, items = __popcll(who) * share;
         for (int it = lane; it < items; it += 64) {
             const int q = it / share, v = (it - q * share) * THREADS + wave * 64 + sh.lane[wave][q];
-            if (v < nv) {
+            if (v < g.nv) {
                 float xs[E::kVec];
-                E::unpack(reinterpret_cast<const u32x4_any*>(x)[v], xs);
+                E::unpack(g.vectors(x)[v], xs);
 #pragma unroll
-                for (int i = 0; i < E::kVec; ++i) collect(xs[i], v * E::kVec + i, !dense);
+                for (int i = 0; i < E::kVec; ++i) collect(xs[i], g.head + v * E::kVec + i, !dense);
             }
         }
-        const int i = nv * E::kVec + tid;
-        if (i < k) collect(E::load(x, i), i, !dense);
+        if (tid < g.extra) collect(E::load(x, g.single(tid)), g.single(tid), !dense);
     }
     __syncthreads();
     const int count = sh.count, above = sh.above, dense = sh.dense;
@@ -373,6 +398,7 @@ __device__ __forceinline__ void block_top(const char* x, int k, int K, float min
         for (int e = tid; e < count; e += THREADS) {
             const uint64_t key = sh.list[e];
             int rank = 0;
+#pragma unroll 8
             for (int j = 0; j < count; ++j) rank += sh.list[j] > key;
             if (rank < K && (!dense || (uint32_t)(key >> 32) > T)) emit(rank, key);
         }
@@ -416,11 +442,13 @@ __global__ __launch_bounds__(THREADS) void log_probs_block_kernel(LogProbsArgs A
     __shared__ BlockShared<THREADS> sh;
     for (int64_t row = blockIdx.x; row < A.n; row += gridDim.x) {
         const char* x = A.x + row * A.row_bytes;
-        float mine;
-        const Stat a = block_stat<TYPE, THREADS, ENT>(x, A.k, A.c, sh, &mine);
-        if (threadIdx.x == 0) write_row<TYPE>(A, row, x, a);
+        const int id = id_of(A, row);
+        const Stat own = block_pass<TYPE, THREADS, ENT>(x, A.k, A.c);
+        const float xid = id >= 0 && threadIdx.x == 0 ? Elem<TYPE>::load(x, id) : 0.f;
+        const Stat a = block_merge(own, A.c, sh);
+        if (threadIdx.x == 0) write_row(A, row, id, xid, a);
         if (A.top)
-            block_top<TYPE>(x, A.k, A.top, mine, a.s != a.s, sh,
+            block_top<TYPE>(x, A.k, A.top, own.m, a.s != a.s, sh,
                             [&](int rank, uint64_t key) { write_top(A, row, rank, key, a); });
         __syncthreads();
     }
@@ -434,14 +462,13 @@ __global__ __launch_bounds__(THREADS) void log_probs_part_kernel(LogProbsArgs A)
     const int64_t row = blockIdx.x, slot = row * A.parts + blockIdx.y;
     const Part p = part_of(A.k, A.parts, blockIdx.y);
     const char* x = A.x + row * A.row_bytes + (int64_t)p.lo * Elem<TYPE>::kSize;
-    float mine;
-    const Stat a = block_stat<TYPE, THREADS, ENT>(x, p.hi - p.lo, A.c, sh, &mine);
+    const Stat own = block_pass<TYPE, THREADS, ENT>(x, p.hi - p.lo, A.c), a = block_merge(own, A.c, sh);
     if (threadIdx.x == 0) A.part_stats[slot] = {a.m, a.s, a.u, 0.f};
     if (A.top) {
         uint64_t* keys = A.part_keys + slot * A.top;
         const int have = min(A.top, p.hi - p.lo);
         for (int r = have + threadIdx.x; r < A.top; r += THREADS) keys[r] = 0;
-        if (have) block_top<TYPE>(x, p.hi - p.lo, have, mine, a.s != a.s, sh,
+        if (have) block_top<TYPE>(x, p.hi - p.lo, have, own.m, a.s != a.s, sh,
                                   [&](int rank, uint64_t key) { keys[rank] = key - p.lo; });
     }
 }
@@ -456,8 +483,10 @@ __global__ __launch_bounds__(64) void log_probs_join_kernel(LogProbsArgs A) {
     __shared__ uint64_t list[64 * kMaxTop];
     const int lane = threadIdx.x;
     const int64_t row = blockIdx.x;
+    const int id = id_of(A, row);
+    const float xid = id >= 0 ? Elem<TYPE>::load(A.x + row * A.row_bytes, id) : 0.f;
     const Stat a = join_stats(A.part_stats + row * A.parts, A.parts, A.c);
-    if (lane == 0) write_row<TYPE>(A, row, A.x + row * A.row_bytes, a);
+    if (lane == 0) write_row(A, row, id, xid, a);
     if (!A.top) return;
     // of every part the first 64 / parts: 64 keys, whose K-th largest is a bound as in block_top
     const uint64_t* keys = A.part_keys + row * A.parts * A.top;
@@ -480,6 +509,7 @@ __global__ __launch_bounds__(64) void log_probs_join_kernel(LogProbsArgs A) {
     for (int e = lane; e < count; e += 64) {
         const uint64_t key = list[e];
         int rank = 0;
+#pragma unroll 8
         for (int j = 0; j < count; ++j) rank += list[j] > key;
         if (rank < A.top) write_top(A, row, rank, key, a);
     }
@@ -492,33 +522,33 @@ template <int TYPE, int THREADS, class F>
 __device__ __forceinline__ void sweep(const char* x, char* dx, int k, F f) {
     using E = Elem<TYPE>;
     constexpr int U = 4, VE = E::kVec;
-    const int nv = k / VE, tid = threadIdx.x, last = nv * VE + tid;
-    if (last < k) E::store(dx, last, f(E::load(x, last)));
-    for (int v0 = (nv - 1) / (U * THREADS) * (U * THREADS); v0 >= 0; v0 -= U * THREADS) {
+    const Grid<TYPE> g(dx, k);
+    const int tid = threadIdx.x;
+    const u32x4_any* from = g.vectors(x);
+    u32x4_any* to = g.vectors(dx);
+    if (tid < g.extra) E::store(dx, g.single(tid), f(E::load(x, g.single(tid))));
+    for (int v0 = (g.nv - 1) / (U * THREADS) * (U * THREADS); v0 >= 0; v0 -= U * THREADS) {
         u32x4 w[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int v = v0 + u * THREADS + tid;
-            if (v < nv) w[u] = reinterpret_cast<const u32x4_any*>(x)[v];
-        }
+        for (int u = 0; u < U; ++u)
+            if (v0 + u * THREADS + tid < g.nv) w[u] = from[v0 + u * THREADS + tid];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int v = v0 + u * THREADS + tid;
             float d[VE];
             E::unpack(w[u], d);
 #pragma unroll
             for (int i = 0; i < VE; ++i) d[i] = f(d[i]);
-            if (v < nv) __builtin_nontemporal_store(E::pack(d), reinterpret_cast<u32x4_any*>(dx) + v);
+            if (v0 + u * THREADS + tid < g.nv) __builtin_nontemporal_store(E::pack(d), to + v0 + u * THREADS + tid);
         }
     }
 }
 // Zeroes a row.
 template <int TYPE, int THREADS>
 __device__ __forceinline__ void clear(char* dx, int k) {
-    using E = Elem<TYPE>;
-    const int nv = k / E::kVec, tid = threadIdx.x, last = nv * E::kVec + tid;
-    for (int v = tid; v < nv; v += THREADS) __builtin_nontemporal_store(u32x4{0, 0, 0, 0}, reinterpret_cast<u32x4_any*>(dx) + v);
-    if (last < k) E::store(dx, last, 0.f);
+    const Grid<TYPE> g(dx, k);
+    const int tid = threadIdx.x;
+    for (int v = tid; v < g.nv; v += THREADS) __builtin_nontemporal_store(u32x4{0, 0, 0, 0}, g.vectors(dx) + v);
+    if (tid < g.extra) Elem<TYPE>::store(dx, g.single(tid), 0.f);
 }
 
 // ---- gradients ---------------------------------------------------------------------------------------------------
@@ -738,10 +768,9 @@ __global__ __launch_bounds__(THREADS) void distill_block_kernel(DistillArgs A) {
     const Part all = {0, A.k};
     for (int64_t row = blockIdx.x; row < A.n; row += gridDim.x) {
         const char* x = A.x + row * A.row_bytes;
-        float mine;
         distill_row<TYPE, THREADS, PER>(A, row, all, sh,
             [&](Teacher<PER>& te) { load_student<TYPE, PER>(te, x, all); },
-            [&] { return block_stat<TYPE, THREADS, false>(x, A.k, A.c, sh, &mine); },
+            [&] { return block_merge(block_pass<TYPE, THREADS, false>(x, A.k, A.c), A.c, sh); },
             [&](float w, const Stat& a) { distill_sweep<TYPE, THREADS>(A, row, all, a, w); });
     }
 }
@@ -759,8 +788,7 @@ __global__ __launch_bounds__(THREADS) void distill_part_kernel(DistillArgs A) {
         const int64_t id = A.ids[row * A.entries + j];
         A.part_x[row * A.entries + j] = id >= 0 && id < A.k ? Elem<TYPE>::load(x, id) : 0.f;
     }
-    float mine;
-    const Stat a = block_stat<TYPE, THREADS, false>(x + (int64_t)p.lo * Elem<TYPE>::kSize, p.hi - p.lo, A.c, sh, &mine);
+    const Stat a = block_merge(block_pass<TYPE, THREADS, false>(x + (int64_t)p.lo * Elem<TYPE>::kSize, p.hi - p.lo, A.c), A.c, sh);
     if (threadIdx.x == 0) A.part_stats[row * A.parts + blockIdx.y] = {a.m, a.s, 0.f, 0.f};
 }
 template <int TYPE, int THREADS, int PER>
@@ -790,22 +818,25 @@ __global__ __launch_bounds__(THREADS) void distill_held_kernel(DistillArgs A) {
     using E = Elem<TYPE>;
     constexpr int VE = E::kVec, U = 2;
     __shared__ BlockShared<THREADS> sh;
-    const int nv = A.k / VE, tid = threadIdx.x, last = nv * VE + tid;
+    const int tid = threadIdx.x;
     const Part all = {0, A.k};
     for (int64_t row = blockIdx.x; row < A.n; row += gridDim.x) {
         const char* x = A.x + row * A.row_bytes;
         char* dx = A.dx + row * A.dx_row_bytes;
+        const Grid<TYPE> g(dx, A.k);
+        const char* from = x + g.head * E::kSize;
+        char* to = dx + g.head * E::kSize;
         u32x4 w[V];
-        float tail = -kInf;
+        float single = -kInf;
         distill_row<TYPE, THREADS, PER>(A, row, all, sh,
             [&](Teacher<PER>& te) { load_student<TYPE, PER>(te, x, all); },
             [&] {
 #pragma unroll
                 for (int u = 0; u < V; ++u) {
                     w[u] = u32x4{E::kNegInf, E::kNegInf, E::kNegInf, E::kNegInf};
-                    if (u * THREADS + tid < nv) w[u] = reinterpret_cast<const u32x4_any*>(x + 16 * u * THREADS)[tid];
+                    if (u * THREADS + tid < g.nv) w[u] = reinterpret_cast<const u32x4_any*>(from + 16 * u * THREADS)[tid];
                 }
-                if (last < A.k) tail = E::load(x, last);
+                if (tid < g.extra) single = E::load(x, g.single(tid));
                 Stat a = {-kInf, 0.f, 0.f};
 #pragma unroll
                 for (int u = 0; u < V; u += U) {
@@ -814,7 +845,7 @@ __global__ __launch_bounds__(THREADS) void distill_held_kernel(DistillArgs A) {
                     for (int i = 0; i < U; ++i) E::unpack(w[u + i], xs + i * VE);
                     accumulate<U * VE, false>(xs, a, A.c);
                 }
-                accumulate<1, false>(&tail, a, A.c);
+                accumulate<1, false>(&single, a, A.c);
                 return block_merge(a, A.c, sh);
             },
             [&](float weight, const Stat& a) {
@@ -830,10 +861,10 @@ __global__ __launch_bounds__(THREADS) void distill_held_kernel(DistillArgs A) {
                     } else {
                         for (int i = 0; i < VE; ++i) d[i] = f * __builtin_amdgcn_exp2f(t_of(d[i]));
                     }
-                    if (u * THREADS + tid < nv)
-                        __builtin_nontemporal_store(E::pack(d), reinterpret_cast<u32x4_any*>(dx + 16 * u * THREADS) + tid);
+                    if (u * THREADS + tid < g.nv)
+                        __builtin_nontemporal_store(E::pack(d), reinterpret_cast<u32x4_any*>(to + 16 * u * THREADS) + tid);
                 }
-                if (last < A.k) E::store(dx, last, f * __builtin_amdgcn_exp2f(t_of(tail)));
+                if (tid < g.extra) E::store(dx, g.single(tid), f * __builtin_amdgcn_exp2f(t_of(single)));
             });
     }
 }
@@ -872,7 +903,11 @@ __global__ __launch_bounds__(64) void log_probs_thread_kernel(LogProbsArgs A) {
         load_short<TYPE, K>(x, A.k, v);
         Stat a = {-kInf, 0.f, 0.f};
         accumulate<K, true>(v, a, A.c);
-        write_row<TYPE>(A, row, x, a);
+        const int id = id_of(A, row);
+        float xid = 0.f;
+#pragma unroll
+        for (int i = 0; i < K; ++i) if (i == id) xid = v[i];
+        write_row(A, row, id, xid, a);
         uint32_t key[K], used = 0;
 #pragma unroll
         for (int i = 0; i < K; ++i) key[i] = score_key(v[i]);
@@ -1019,16 +1054,20 @@ __device__ __forceinline__ void wave_top(const float* v, int k, int K, float min
 template <int TYPE, int N, bool ENT>
 __global__ __launch_bounds__(256) void log_probs_wave_kernel(LogProbsArgs A) {
     __shared__ uint64_t list[4][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     for (int64_t row = (int64_t)blockIdx.x * 4 + wave; row < A.n; row += (int64_t)gridDim.x * 4) {
         const char* x = A.x + row * A.row_bytes;
         float v[N];
+        const int id = id_of(A, row);
         load_spread<TYPE, N>(x, A.k, v);
         Stat a = {-kInf, 0.f, 0.f};
         accumulate<N, ENT>(v, a, A.c);
         const float mine = a.m;
         a = wave_merge(a, A.c);
-        if (lane == 0) write_row<TYPE>(A, row, x, a);
+        float xid = 0.f;
+#pragma unroll
+        for (int j = 0; j < N; ++j) if (id >> 6 == j) xid = lane_of(v[j], id & 63);
+        if (lane == 0) write_row(A, row, id, xid, a);
         if (A.top)
             wave_top<TYPE, N>(v, A.k, A.top, mine, a.s != a.s, list[wave],
                               [&](int rank, uint64_t key) { write_top(A, row, rank, key, a); });
@@ -1038,7 +1077,7 @@ __global__ __launch_bounds__(256) void log_probs_wave_kernel(LogProbsArgs A) {
 template <int TYPE, int N>
 __global__ __launch_bounds__(256) void log_probs_grad_wave_kernel(LogProbsGradArgs A) {
     const int lane = threadIdx.x & 63;
-    for (int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); row < A.n; row += (int64_t)gridDim.x * 4) {
+    for (int64_t row = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); row < A.n; row += (int64_t)gridDim.x * 4) {
         const float m = A.stats[2 * row], s = A.stats[2 * row + 1];
         float v[N];
         load_spread<TYPE, N>(A.x + row * A.row_bytes, A.k, v);
@@ -1056,7 +1095,7 @@ __global__ __launch_bounds__(256) void log_probs_grad_wave_kernel(LogProbsGradAr
 template <int TYPE, int N, int PER>
 __global__ __launch_bounds__(256) void distill_wave_kernel(DistillArgs A) {
     const int lane = threadIdx.x & 63;
-    for (int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); row < A.n; row += (int64_t)gridDim.x * 4) {
+    for (int64_t row = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); row < A.n; row += (int64_t)gridDim.x * 4) {
         const char* x = A.x + row * A.row_bytes;
         char* dx = A.dx + row * A.dx_row_bytes;
         float w = A.weights ? A.weights[row] : 1.f;
@@ -1098,16 +1137,21 @@ __global__ __launch_bounds__(256) void distill_wave_kernel(DistillArgs A) {
 constexpr int64_t kMaxGrid = 1 << 20;       // workgroups of a launch; further rows are taken by a loop
 unsigned row_grid(int64_t n) { return (unsigned)std::min(n, kMaxGrid); }
 
+int elem_size(int type) { return type == CD_T_F32 ? 4 : 2; }
+
 // Threads of a workgroup that reads a row of more than kWaveClasses scores: many for few rows, since a row's time is then
 // what counts; else as few as keep a few pieces of 64 bytes per thread, so that several rows share a CU and one's reads
 // fill another's waits (4096 rows, 20 alternatives: 8000 x bf16 27 us with 256 threads, 42 with 512, 111 with 1024; 128000 x
-// bf16 263, 217 and 249; 64 rows of 131072 x bf16: 29, 19 and 16).
+// bf16 263, 217 and 249; 64 rows of 131072 x bf16: 29, 19 and 16).  Where 256 threads, six workgroups to a CU, hold all rows
+// at once and 512, three, would need a second round: 256 (1000 x 50021 f32: 39 us against 44).
 int block_threads(const RowsIn& in) {
 #ifdef CD_EXP_ENV
     if (const char* e = std::getenv("CUTDET_X_THREADS")) return std::atoi(e);
 #endif
-    const int64_t bytes = (int64_t)in.k * (in.type == CD_T_F32 ? 4 : 2);
-    return bytes <= 32768 ? 256 : in.n <= 256 && bytes > 65536 ? 1024 : 512;
+    const int64_t bytes = (int64_t)in.k * elem_size(in.type);
+    if (bytes <= 32768) return 256;
+    if (in.n <= 256 && bytes > 65536) return 1024;
+    return in.n > 768 && in.n <= 1536 ? 256 : 512;
 }
 
 // CALL(type, ...) for the type of the scores
@@ -1120,7 +1164,6 @@ int block_threads(const RowsIn& in) {
 
 unsigned thread_grid(int64_t n) { return row_grid((n + 63) / 64); }
 unsigned wave_grid(int64_t n) { return row_grid((n + 3) / 4); }
-int elem_size(int type) { return type == CD_T_F32 ? 4 : 2; }
 constexpr int64_t kSplitBytes = 128 << 10, kSplitRows = 64;
 
 }  // namespace
@@ -1245,10 +1288,10 @@ int launch_distill(const RowsIn& in, const TeacherIn& te, float* stats, float* l
     else distill_held_kernel<TY, TH, V, kMaxTeacher / 64><<<row_grid(in.n), TH, 0, s>>>(A)
         const int vectors = in.k / (16 / elem_size(in.type));
         if (A.parts > 1) CD_BY_TYPE(in.type, PARTS, 512);
-        else if (vectors <= 256 * 8) CD_BY_TYPE(in.type, HELD, 256, 8);
-        else if (vectors <= 512 * 8) CD_BY_TYPE(in.type, HELD, 512, 8);
-        else if (vectors <= 512 * 16) CD_BY_TYPE(in.type, HELD, 512, 16);
-        else if (vectors <= 1024 * 16) CD_BY_TYPE(in.type, HELD, 1024, 16);
+        else if (dx && vectors <= 256 * 8) CD_BY_TYPE(in.type, HELD, 256, 8);
+        else if (dx && vectors <= 512 * 8) CD_BY_TYPE(in.type, HELD, 512, 8);
+        else if (dx && vectors <= 512 * 16) CD_BY_TYPE(in.type, HELD, 512, 16);
+        else if (dx && vectors <= 1024 * 16) CD_BY_TYPE(in.type, HELD, 1024, 16);
         else if (block_threads(in) == 256) CD_BY_TYPE(in.type, BLOCK, 256);
         else if (block_threads(in) == 512) CD_BY_TYPE(in.type, BLOCK, 512);
         else CD_BY_TYPE(in.type, BLOCK, 1024);

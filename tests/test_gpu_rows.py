@@ -239,8 +239,9 @@ def check_distill(eng, x, ids, te, w=None, t=1.0):
     alone = eng.distill(x, ids, te, w, t)
     assert "grad" not in alone
     both = eng.distill(x, ids, te, w, t, grad=True)
+    # (not bit for bit: the two calls may add the same terms in another order; each has to be within the bound)
     ref.check_loss(alone["loss"], loss, size, k)
-    assert torch.equal(alone["loss"].view(torch.int32), both["loss"].view(torch.int32))
+    ref.check_loss(both["loss"], loss, size, k)
     ref.check_grad(both["grad"], grad, gsize, k)
     g = vector(x.shape[0], 8)
     late = eng.distill_backward(x, ids, te, alone["stats"], g, w, t)
@@ -489,9 +490,9 @@ def test_a_teachers_alternatives_train_a_student(eng, k):
     before = losses.distill_loss(x, t["top_ids"], t["top_logp"]).detach()
     both = eng.distill(x.detach(), t["top_ids"], t["top_logp"], grad=True)
     losses.distill_loss(x, t["top_ids"], t["top_logp"]).sum().backward()
-    assert torch.equal(both["grad"], x.grad) and torch.equal(both["loss"], before)
     want = ref.distill64(x.detach(), t["top_ids"], t["top_logp"])
-    ref.check_loss(before, want[0], want[1], k)
-    ref.check_grad(x.grad, want[2], want[3], k)
+    for loss, grad in ((before, x.grad), (both["loss"], both["grad"])):
+        ref.check_loss(loss, want[0], want[1], k)
+        ref.check_grad(grad, want[2], want[3], k)
     after = eng.distill(x.detach() - 0.1 * x.grad, t["top_ids"], t["top_logp"])["loss"]
     assert (after < before).all()            # a descent step of a convex function with curvature below 1
