@@ -89,10 +89,16 @@ template <> struct Elem<CD_T_F16> {
     }
 };
 
+// a score of a type known at run time: its bits, which the caller may leave in flight, and their value
+__device__ __forceinline__ uint32_t load_bits(int type, const void* p, int64_t i) {
+    return type == CD_T_F32 ? static_cast<const uint32_t*>(p)[i] : static_cast<const uint16_t*>(p)[i];
+}
+__device__ __forceinline__ float bits_value(int type, uint32_t b) {
+    return type == CD_T_F32 ? __uint_as_float(b) : type == CD_T_BF16 ? __uint_as_float(b << 16)
+         : (float)__builtin_bit_cast(_Float16, (uint16_t)b);
+}
 __device__ __forceinline__ float load_any(int type, const void* p, int64_t i) {
-    const char* row = static_cast<const char*>(p);
-    return type == CD_T_F32 ? Elem<CD_T_F32>::load(row, i)
-         : type == CD_T_BF16 ? Elem<CD_T_BF16>::load(row, i) : Elem<CD_T_F16>::load(row, i);
+    return bits_value(type, load_bits(type, p, i));
 }
 
 // ---- wave reductions on the DPP network; the result is uniform ---------------------------------------------------
@@ -618,8 +624,10 @@ struct DistillArgs {
     float* part_x;
 };
 template <int PER> struct Teacher { // the entries of one row, spread over a wave: entry lane + 64 e, e < PER
+    int64_t raw_id[PER];            // as loaded
+    uint32_t raw_score[PER];
     int id[PER];                    // -1: unused
-    float lq[PER];                  // the teacher's score, then log2 q
+    float lq[PER];                  // log2 q
     float q[PER];
     float sum[PER];                 // of a class named more than once: its q's together at its first entry, else -1
     float x[PER];                   // the student's score
@@ -631,15 +639,12 @@ __device__ __forceinline__ void load_entries(Teacher<PER>& r, const DistillArgs&
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
         const int j = lane + 64 * e;
-        int64_t id = -1;
-        float v = -kInf;
+        r.raw_id[e] = -1;
+        r.raw_score[e] = 0;
         if (j < A.entries) {
-            id = A.ids[row * A.entries + j];
-            v = load_any(A.teacher_type, A.teacher, row * A.entries + j);
+            r.raw_id[e] = A.ids[row * A.entries + j];
+            r.raw_score[e] = load_bits(A.teacher_type, A.teacher, row * A.entries + j);
         }
-        const bool used = id >= 0 && id < A.k;
-        r.id[e] = used ? (int)id : -1;
-        r.lq[e] = used ? v : -kInf;
     }
 }
 template <int PER>
@@ -647,7 +652,12 @@ __device__ __forceinline__ void share_out(Teacher<PER>& r, const DistillArgs& A)
     const int lane = threadIdx.x & 63;
     float m = -kInf, total = 0.f;
 #pragma unroll
-    for (int e = 0; e < PER; ++e) m = fmaxf(m, r.lq[e]);
+    for (int e = 0; e < PER; ++e) {
+        const bool used = r.raw_id[e] >= 0 && r.raw_id[e] < A.k;
+        r.id[e] = used ? (int)r.raw_id[e] : -1;
+        r.lq[e] = used ? bits_value(A.teacher_type, r.raw_score[e]) : -kInf;
+        m = fmaxf(m, r.lq[e]);
+    }
     m = wave_max(m);
     const Ref t_of(m, A.c);
 #pragma unroll
@@ -658,24 +668,45 @@ __device__ __forceinline__ void share_out(Teacher<PER>& r, const DistillArgs& A)
     }
     r.total = wave_sum(total);
     const float l = __builtin_amdgcn_logf(r.total), inv = 1.f / r.total;
-    bool first[PER];
 #pragma unroll
-    for (int e = 0; e < PER; ++e) { r.lq[e] -= l; r.q[e] *= inv; r.sum[e] = 0.f; first[e] = r.id[e] >= 0; }
-    if (A.dx) {
+    for (int e = 0; e < PER; ++e) { r.lq[e] -= l; r.q[e] *= inv; r.sum[e] = r.id[e] >= 0 ? r.q[e] : -1.f; }
+    if (!A.dx) return;
+    // entries of the same class: same[e][f] are the lanes whose entry f names the class of this lane's entry e, found bit
+    // by bit of the class
+    uint64_t same[PER][PER];
 #pragma unroll
-        for (int f = 0; f < PER; ++f)
-            for (int l = 0; l < min(64, A.entries - 64 * f); ++l) {
-                const int id = __builtin_amdgcn_readlane(r.id[f], l);
-                const float q = lane_of(r.q[f], l);
+    for (int e = 0; e < PER; ++e)
 #pragma unroll
-                for (int e = 0; e < PER; ++e)
-                    if (id == r.id[e]) {
-                        r.sum[e] += q;
-                        if (64 * f + l < 64 * e + lane) first[e] = false;
-                    }
+        for (int f = 0; f < PER; ++f) same[e][f] = __ballot(r.id[f] >= 0);
+    for (int b = 0; (A.k - 1) >> b; ++b)
+#pragma unroll
+        for (int f = 0; f < PER; ++f) {
+            const uint64_t ones = __ballot(r.id[f] >> b & 1);
+#pragma unroll
+            for (int e = 0; e < PER; ++e) same[e][f] &= r.id[e] >> b & 1 ? ones : ~ones;
+        }
+    bool again = false;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+        int count = 0;
+#pragma unroll
+        for (int f = 0; f < PER; ++f) count += __popcll(same[e][f]);
+        again |= r.id[e] >= 0 && count > 1;
+    }
+    if (!__any(again)) return;                            // no class twice
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+        float sum = 0.f;
+        bool first = r.id[e] >= 0;
+#pragma unroll
+        for (int f = 0; f < PER; ++f) {
+            if (first && (f < e ? same[e][f] != 0 : f == e && (same[e][e] & ((1ull << lane) - 1)))) first = false;
+            for (uint64_t left = r.id[e] >= 0 ? same[e][f] : 0; __any(left != 0); left &= left - 1) {
+                const float q = __shfl(r.q[f], left ? __ffsll((unsigned long long)left) - 1 : lane);
+                if (left) sum += q;
             }
-#pragma unroll
-        for (int e = 0; e < PER; ++e) if (!first[e]) r.sum[e] = -1.f;
+        }
+        r.sum[e] = first ? sum : -1.f;
     }
 }
 template <int TYPE, int PER>
@@ -723,10 +754,10 @@ __device__ __forceinline__ void distill_sweep(const DistillArgs& A, int64_t row,
 
 // What the kernels below share: the row's weight, its teacher (wave 0; every thread learns whether an entry counts), its
 // statistics from `pass`, the loss (part 0), and the gradient of part p from `grad(w, a)`, which writes w T p of every
-// class.  `student` loads the student's scores of the teacher's classes.
-template <int TYPE, int THREADS, int PER, class Student, class Pass, class Grad>
+// class.  `load` may start loads that `pass` uses; `student` loads the student's scores of the teacher's classes.
+template <int TYPE, int THREADS, int PER, class Load, class Student, class Pass, class Grad>
 __device__ __forceinline__ void distill_row(const DistillArgs& A, int64_t row, Part p, BlockShared<THREADS>& sh,
-                                            Student student, Pass pass, Grad grad) {
+                                            Load load, Student student, Pass pass, Grad grad) {
     char* dx = A.dx + row * A.dx_row_bytes;
     const int tid = threadIdx.x;
     float w = A.weights ? A.weights[row] : 1.f;
@@ -735,8 +766,9 @@ __device__ __forceinline__ void distill_row(const DistillArgs& A, int64_t row, P
     Teacher<PER> te;
     bool on = false;
     if (w != 0.f) {
+        if (tid < 64) load_entries<PER>(te, A, row);      // (in flight before the row's own loads, if `load` makes them)
+        load();
         if (tid < 64) {
-            load_entries<PER>(te, A, row);
             share_out<PER>(te, A);
             student(te);
             if (tid == 0) sh.total = te.total;
@@ -768,7 +800,7 @@ __global__ __launch_bounds__(THREADS) void distill_block_kernel(DistillArgs A) {
     const Part all = {0, A.k};
     for (int64_t row = blockIdx.x; row < A.n; row += gridDim.x) {
         const char* x = A.x + row * A.row_bytes;
-        distill_row<TYPE, THREADS, PER>(A, row, all, sh,
+        distill_row<TYPE, THREADS, PER>(A, row, all, sh, [] {},
             [&](Teacher<PER>& te) { load_student<TYPE, PER>(te, x, all); },
             [&] { return block_merge(block_pass<TYPE, THREADS, false>(x, A.k, A.c), A.c, sh); },
             [&](float w, const Stat& a) { distill_sweep<TYPE, THREADS>(A, row, all, a, w); });
@@ -796,7 +828,7 @@ __global__ __launch_bounds__(THREADS) void distill_join_kernel(DistillArgs A) {
     __shared__ BlockShared<THREADS> sh;
     const int64_t row = blockIdx.x;
     const Part p = part_of(A.k, gridDim.y, blockIdx.y);   // (grid y is 1 where there is no gradient)
-    distill_row<TYPE, THREADS, PER>(A, row, p, sh,
+    distill_row<TYPE, THREADS, PER>(A, row, p, sh, [] {},
         [&](Teacher<PER>& te) {
 #pragma unroll
             for (int e = 0; e < PER; ++e) {
@@ -829,7 +861,6 @@ __global__ __launch_bounds__(THREADS) void distill_held_kernel(DistillArgs A) {
         u32x4 w[V];
         float single = -kInf;
         distill_row<TYPE, THREADS, PER>(A, row, all, sh,
-            [&](Teacher<PER>& te) { load_student<TYPE, PER>(te, x, all); },
             [&] {
 #pragma unroll
                 for (int u = 0; u < V; ++u) {
@@ -837,6 +868,9 @@ __global__ __launch_bounds__(THREADS) void distill_held_kernel(DistillArgs A) {
                     if (u * THREADS + tid < g.nv) w[u] = reinterpret_cast<const u32x4_any*>(from + 16 * u * THREADS)[tid];
                 }
                 if (tid < g.extra) single = E::load(x, g.single(tid));
+            },
+            [&](Teacher<PER>& te) { load_student<TYPE, PER>(te, x, all); },
+            [&] {
                 Stat a = {-kInf, 0.f, 0.f};
 #pragma unroll
                 for (int u = 0; u < V; u += U) {
@@ -876,7 +910,7 @@ __global__ __launch_bounds__(THREADS) void distill_grad_kernel(DistillArgs A) {
     const Part p = part_of(A.k, gridDim.y, blockIdx.y);
     for (int64_t back = blockIdx.x; back < A.n; back += gridDim.x) {
         const int64_t row = A.n - 1 - back;
-        distill_row<TYPE, THREADS, PER>(A, row, p, sh,
+        distill_row<TYPE, THREADS, PER>(A, row, p, sh, [] {},
             [&](Teacher<PER>& te) { load_student<TYPE, PER>(te, A.x + row * A.row_bytes, p); },
             [&] {
                 __syncthreads();
@@ -1252,12 +1286,19 @@ static DistillArgs distill_args(const RowsIn& in, const TeacherIn& te, float* st
             loss};
 }
 
+// by the entries that a lane of the wave that looks after the teacher has
+#define PER_LANE(ONE, TWO, FOUR)              \
+    if (A.entries <= 64) { ONE; }             \
+    else if (A.entries <= 128) { TWO; }       \
+    else { FOUR; }
+
 // rows of up to kWaveClasses scores, which the gradient alone computes anew; false: longer ones
 static bool launch_short_distill(const RowsIn& in, const DistillArgs& A, hipStream_t s) {
 #define SHORT(TY, K) distill_thread_kernel<TY, K><<<thread_grid(in.n), 64, 0, s>>>(A)
 #define WAVE(TY, N)                                                                                \
-    if (A.entries <= 64) distill_wave_kernel<TY, N, 1><<<wave_grid(in.n), 256, 0, s>>>(A);         \
-    else distill_wave_kernel<TY, N, kMaxTeacher / 64><<<wave_grid(in.n), 256, 0, s>>>(A)
+    PER_LANE((distill_wave_kernel<TY, N, 1><<<wave_grid(in.n), 256, 0, s>>>(A)),                     \
+             (distill_wave_kernel<TY, N, 2><<<wave_grid(in.n), 256, 0, s>>>(A)),                     \
+             (distill_wave_kernel<TY, N, 4><<<wave_grid(in.n), 256, 0, s>>>(A)))
     if (in.k <= 4 && A.entries <= 16) CD_BY_TYPE(in.type, SHORT, 4);
     else if (in.k <= kThreadClasses && A.entries <= 16) CD_BY_TYPE(in.type, SHORT, kThreadClasses);
     else if (in.k <= 256) CD_BY_TYPE(in.type, WAVE, 4);
@@ -1278,14 +1319,17 @@ int launch_distill(const RowsIn& in, const TeacherIn& te, float* stats, float* l
     if (!launch_short_distill(in, A, s)) {
 #define PARTS(TY, TH)                                                                                       \
     distill_part_kernel<TY, TH><<<parts, TH, 0, s>>>(A);                                                    \
-    if (A.entries <= 64) distill_join_kernel<TY, 256, 1><<<writers, 256, 0, s>>>(A);                        \
-    else distill_join_kernel<TY, 256, kMaxTeacher / 64><<<writers, 256, 0, s>>>(A)
+    PER_LANE((distill_join_kernel<TY, 256, 1><<<writers, 256, 0, s>>>(A)),                                    \
+             (distill_join_kernel<TY, 256, 2><<<writers, 256, 0, s>>>(A)),                                    \
+             (distill_join_kernel<TY, 256, 4><<<writers, 256, 0, s>>>(A)))
 #define BLOCK(TY, TH)                                                                                       \
-    if (A.entries <= 64) distill_block_kernel<TY, TH, 1><<<row_grid(in.n), TH, 0, s>>>(A);                  \
-    else distill_block_kernel<TY, TH, kMaxTeacher / 64><<<row_grid(in.n), TH, 0, s>>>(A)
+    PER_LANE((distill_block_kernel<TY, TH, 1><<<row_grid(in.n), TH, 0, s>>>(A)),                              \
+             (distill_block_kernel<TY, TH, 2><<<row_grid(in.n), TH, 0, s>>>(A)),                              \
+             (distill_block_kernel<TY, TH, 4><<<row_grid(in.n), TH, 0, s>>>(A)))
 #define HELD(TY, TH, V)                                                                                     \
-    if (A.entries <= 64) distill_held_kernel<TY, TH, V, 1><<<row_grid(in.n), TH, 0, s>>>(A);                \
-    else distill_held_kernel<TY, TH, V, kMaxTeacher / 64><<<row_grid(in.n), TH, 0, s>>>(A)
+    PER_LANE((distill_held_kernel<TY, TH, V, 1><<<row_grid(in.n), TH, 0, s>>>(A)),                          \
+             (distill_held_kernel<TY, TH, V, 2><<<row_grid(in.n), TH, 0, s>>>(A)),                          \
+             (distill_held_kernel<TY, TH, V, 4><<<row_grid(in.n), TH, 0, s>>>(A)))
         const int vectors = in.k / (16 / elem_size(in.type));
         if (A.parts > 1) CD_BY_TYPE(in.type, PARTS, 512);
         else if (dx && vectors <= 256 * 8) CD_BY_TYPE(in.type, HELD, 256, 8);
@@ -1310,8 +1354,9 @@ int launch_distill_backward(const RowsIn& in, const TeacherIn& te, const float* 
         A.stats = const_cast<float*>(stats);              // only read
         const dim3 grid(row_grid(in.n), grad_parts(in.n, in.k, in.type));
 #define BLOCK(TY, TH)                                                                                       \
-    if (A.entries <= 64) distill_grad_kernel<TY, TH, 1><<<grid, TH, 0, s>>>(A);                             \
-    else distill_grad_kernel<TY, TH, kMaxTeacher / 64><<<grid, TH, 0, s>>>(A)
+    PER_LANE((distill_grad_kernel<TY, TH, 1><<<grid, TH, 0, s>>>(A)),                                         \
+             (distill_grad_kernel<TY, TH, 2><<<grid, TH, 0, s>>>(A)),                                         \
+             (distill_grad_kernel<TY, TH, 4><<<grid, TH, 0, s>>>(A)))
         CD_BY_TYPE(in.type, BLOCK, 256);
 #undef BLOCK
     }
