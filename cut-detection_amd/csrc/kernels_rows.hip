@@ -1022,128 +1022,212 @@ __global__ __launch_bounds__(64) void distill_thread_kernel(DistillArgs A) {
     }
 }
 
-// ================================================================================== one wave per row, up to 1024 scores
-// Score i is in lane i % 64, so the order of the classes is the order of (register, lane).
-constexpr int kWaveClasses = 1024;
+// ================================================================================== one wave per row, up to 4096 scores
+// The row stays in the wave's registers, no barrier, and four rows to a workgroup: 30000 x 2000 bf16 with 20 alternatives
+// takes 61 us so and 152 us with a workgroup per row, 30000 x 4000 loss and gradient 100 us and 183 us.  Beyond 2048
+// scores (log_probs: its alternatives) or 8 KB the registers leave too few waves.  Up to 512 scores one score at a time, score i in lane
+// i % 64; above that vectors of 16 bytes, so that every lane has some, and the rest of a row one score per lane (50000 x
+// 1000 bf16: 32 us with vectors, 83 us without).
+constexpr int kWaveClasses = 2048, kWaveBytes = 8192;
 
-template <int TYPE, int N>
-__device__ __forceinline__ void load_spread(const char* x, int k, float* v) {
-    const int lane = threadIdx.x & 63;
+template <int TYPE, int N> struct SpreadRow {
+    static constexpr int kCount = N;                      // scores of a lane
+    float v[N];
+    int k;
+    __device__ __forceinline__ void load(const char* x, int k_) {
+        k = k_;
 #pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = lane + 64 * j < k ? Elem<TYPE>::load(x, lane + 64 * j) : -kInf;
-}
+        for (int j = 0; j < N; ++j) v[j] = index(j) < k ? Elem<TYPE>::load(x, index(j)) : -kInf;
+    }
+    __device__ __forceinline__ int index(int j) const { return (threadIdx.x & 63) + 64 * j; }
+    __device__ __forceinline__ bool valid(int j) const { return index(j) < k; }
+    __device__ __forceinline__ float value(int j) const { return v[j]; }
+    __device__ __forceinline__ void pin() {}
+    template <bool ENT> __device__ __forceinline__ void add(Stat& a, float c) const { accumulate<N, ENT>(v, a, c); }
+    __device__ __forceinline__ float at(int id) const {   // of a uniform id
+        float r = 0.f;
+#pragma unroll
+        for (int j = 0; j < N; ++j) if (id >> 6 == j) r = lane_of(v[j], id & 63);
+        return r;
+    }
+    template <class F> __device__ __forceinline__ void write(char* dx, F f) const {
+#pragma unroll
+        for (int j = 0; j < N; ++j) if (valid(j)) Elem<TYPE>::store(dx, index(j), f(v[j]));
+    }
+};
+template <int TYPE, int V> struct VectorRow {
+    using E = Elem<TYPE>;
+    static constexpr int kCount = V * E::kVec + 1;
+    u32x4 w[V];
+    float single;
+    const char* x;
+    int k, nv;
+    __device__ __forceinline__ void load(const char* x_, int k_) {
+        x = x_;
+        k = k_;
+        nv = k / E::kVec;
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int u = 0; u < V; ++u) {
+            w[u] = u32x4{E::kNegInf, E::kNegInf, E::kNegInf, E::kNegInf};
+            if (lane + 64 * u < nv) w[u] = reinterpret_cast<const u32x4_any*>(x + 1024 * u)[lane];
+        }
+        single = nv * E::kVec + lane < k ? E::load(x, nv * E::kVec + lane) : -kInf;
+    }
+    __device__ __forceinline__ int index(int j) const {
+        const int lane = threadIdx.x & 63;
+        return j == V * E::kVec ? nv * E::kVec + lane : (lane + 64 * (j / E::kVec)) * E::kVec + j % E::kVec;
+    }
+    __device__ __forceinline__ bool valid(int j) const {
+        return j == V * E::kVec ? index(j) < k : (int)(threadIdx.x & 63) + 64 * (j / E::kVec) < nv;
+    }
+    __device__ __forceinline__ float value(int j) const {
+        if (j == V * E::kVec) return single;
+        float xs[E::kVec];
+        E::unpack(w[j / E::kVec], xs);
+        return xs[j % E::kVec];
+    }
+    template <bool ENT> __device__ __forceinline__ void add(Stat& a, float c) const {
+        constexpr int U = V < 4 ? V : 4;
+#pragma unroll
+        for (int u = 0; u < V; u += U) {
+            float xs[U * E::kVec];
+#pragma unroll
+            for (int i = 0; i < U; ++i) E::unpack(w[u + i], xs + i * E::kVec);
+            accumulate<U * E::kVec, ENT>(xs, a, c);
+        }
+        accumulate<1, ENT>(&single, a, c);
+    }
+    // keeps the compiler from unpacking the row outside a loop, which takes twice the registers
+    __device__ __forceinline__ void pin() {
+#pragma unroll
+        for (int u = 0; u < V; ++u) asm volatile("" : "+v"(w[u]));
+    }
+    __device__ __forceinline__ float at(int id) const { return E::load(x, id); }
+    template <class F> __device__ __forceinline__ void write(char* dx, F f) const {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int u = 0; u < V; ++u) {
+            float d[E::kVec];
+            E::unpack(w[u], d);
+#pragma unroll
+            for (int i = 0; i < E::kVec; ++i) d[i] = f(d[i]);
+            if (lane + 64 * u < nv) reinterpret_cast<u32x4_any*>(dx + 1024 * u)[lane] = E::pack(d);
+        }
+        if (nv * E::kVec + lane < k) E::store(dx, nv * E::kVec + lane, f(single));
+    }
+};
 
-// As block_top; where more than 64 scores reach T (equal ones), the K-th largest score itself takes the place of T, and
-// of those equal to it the lowest classes count.
-template <int TYPE, int N, class Emit>
-__device__ __forceinline__ void wave_top(const float* v, int k, int K, float mine, bool nan, uint64_t* list, Emit emit) {
+// As block_top, from the registers; where more than 64 scores reach T (equal ones), and for NaN, the K-th largest key
+// itself takes the place of T.
+template <class Row, class Emit>
+__device__ __forceinline__ void wave_top(Row& r, int K, float mine, bool nan, uint64_t* list, Emit emit) {
     const int lane = threadIdx.x & 63;
     const uint64_t below = (1ull << lane) - 1;
-    uint32_t key[N], high = 0;
-#pragma unroll
-    for (int j = 0; j < N; ++j) key[j] = lane + 64 * j < k ? score_key(v[j]) : 0;
-    if (nan) {
-#pragma unroll
-        for (int j = 0; j < N; ++j) high = key[j] > high ? key[j] : high;
-    } else if (lane < k) high = score_key(mine);
-    uint32_t t = kth_key<0>(high, K);
     int count = 0;
+    r.pin();
+    if (!nan) {
+        const float t = key_score(kth_key<0>(score_key(mine), K));
 #pragma unroll
-    for (int j = 0; j < N; ++j) count += __popcll(__ballot(key[j] >= t));
-    int ties = 64;                                        // of the scores at t, as many as there are
-    if (count > 64) {
-        t = 0;
-        for (int b = 31; b >= 0; --b) {
-            const uint32_t up = t | 1u << b;
+        for (int j = 0; j < Row::kCount; ++j) {
+            const bool take = r.value(j) >= t && r.valid(j);
+            const uint64_t taken = __ballot(take);
+            if (taken) {
+                const int at = count + __popcll(taken & below);
+                if (take && at < 64) list[at] = full_key(r.value(j), r.index(j));
+                count += __popcll(taken);
+            }
+        }
+    }
+    if (nan || count > 64) {
+        uint64_t t = 0;
+        for (int b = 63; b >= 0; --b) {
+            const uint64_t up = t | 1ull << b;
             int c = 0;
+            r.pin();
 #pragma unroll
-            for (int j = 0; j < N; ++j) c += __popcll(__ballot(key[j] >= up));
+            for (int j = 0; j < Row::kCount; ++j)
+                c += __popcll(__ballot(r.valid(j) && full_key(r.value(j), r.index(j)) >= up));
             if (c >= K) t = up;
         }
-        int above = 0;
+        count = 0;
+        r.pin();
 #pragma unroll
-        for (int j = 0; j < N; ++j) above += __popcll(__ballot(key[j] > t));
-        ties = K - above;
-    }
-    count = 0;
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-        const uint64_t equal = __ballot(key[j] == t), up = __ballot(key[j] > t);
-        const bool take = up >> lane & 1 || (equal >> lane & 1 && __popcll(equal & below) < ties);
-        const uint64_t taken = __ballot(take);
-        if (take) list[count + __popcll(taken & below)] = (uint64_t)key[j] << 32 | (uint32_t)~(lane + 64 * j);
-        count += __popcll(taken);
-        ties -= min(ties, __popcll(equal));
+        for (int j = 0; j < Row::kCount; ++j) {
+            const uint64_t key = full_key(r.value(j), r.index(j));
+            const bool take = r.valid(j) && key >= t;
+            const uint64_t taken = __ballot(take);
+            if (take) list[count + __popcll(taken & below)] = key;
+            count += __popcll(taken);
+        }
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     if (lane < count) {
         const uint64_t mykey = list[lane];
         int rank = 0;
+#pragma unroll 4
         for (int j = 0; j < count; ++j) rank += list[j] > mykey;
         if (rank < K) emit(rank, mykey);
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 }
 
-template <int TYPE, int N, bool ENT>
+template <class Row, bool ENT>
 __global__ __launch_bounds__(256) void log_probs_wave_kernel(LogProbsArgs A) {
     __shared__ uint64_t list[4][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     for (int64_t row = (int64_t)blockIdx.x * 4 + wave; row < A.n; row += (int64_t)gridDim.x * 4) {
-        const char* x = A.x + row * A.row_bytes;
-        float v[N];
         const int id = id_of(A, row);
-        load_spread<TYPE, N>(x, A.k, v);
+        Row r;
+        r.load(A.x + row * A.row_bytes, A.k);
+        const float xid = id >= 0 ? r.at(id) : 0.f;
         Stat a = {-kInf, 0.f, 0.f};
-        accumulate<N, ENT>(v, a, A.c);
+        r.template add<ENT>(a, A.c);
         const float mine = a.m;
         a = wave_merge(a, A.c);
-        float xid = 0.f;
-#pragma unroll
-        for (int j = 0; j < N; ++j) if (id >> 6 == j) xid = lane_of(v[j], id & 63);
         if (lane == 0) write_row(A, row, id, xid, a);
         if (A.top)
-            wave_top<TYPE, N>(v, A.k, A.top, mine, a.s != a.s, list[wave],
-                              [&](int rank, uint64_t key) { write_top(A, row, rank, key, a); });
+            wave_top(r, A.top, mine, a.s != a.s, list[wave], [&](int rank, uint64_t key) { write_top(A, row, rank, key, a); });
     }
 }
 
-template <int TYPE, int N>
+template <class Row, int TYPE>
 __global__ __launch_bounds__(256) void log_probs_grad_wave_kernel(LogProbsGradArgs A) {
     const int lane = threadIdx.x & 63;
-    for (int64_t row = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); row < A.n; row += (int64_t)gridDim.x * 4) {
+    for (int64_t row = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); row < A.n;
+         row += (int64_t)gridDim.x * 4) {
+        char* dx = A.dx + row * A.dx_row_bytes;
+        Row r;
+        r.load(A.x + row * A.row_bytes, A.k);
         const float m = A.stats[2 * row], s = A.stats[2 * row + 1];
-        float v[N];
-        load_spread<TYPE, N>(A.x + row * A.row_bytes, A.k, v);
         const GradRow g = grad_row(A, row, s);
         const Ref t_of(m, A.c);
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const int i = lane + 64 * j;
-            if (i < A.k)
-                Elem<TYPE>::store(A.dx + row * A.dx_row_bytes, i, grad_of(t_of(v[j]), g) + (i == g.id ? g.hit : 0.f));
-        }
+        const float hit = g.id >= 0 ? grad_of(t_of(r.at(g.id)), g) + g.hit : 0.f;
+        r.write(dx, [&](float v) { return grad_of(t_of(v), g); });
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");          // the row first, then its class
+        if (lane == 0 && g.id >= 0) Elem<TYPE>::store(dx, g.id, hit);
     }
 }
 
-template <int TYPE, int N, int PER>
+template <class Row, int TYPE, int PER>
 __global__ __launch_bounds__(256) void distill_wave_kernel(DistillArgs A) {
     const int lane = threadIdx.x & 63;
-    for (int64_t row = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); row < A.n; row += (int64_t)gridDim.x * 4) {
+    for (int64_t row = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); row < A.n;
+         row += (int64_t)gridDim.x * 4) {
         const char* x = A.x + row * A.row_bytes;
         char* dx = A.dx + row * A.dx_row_bytes;
         float w = A.weights ? A.weights[row] : 1.f;
         if (A.g_loss && w != 0.f) w *= A.g_loss[row];
-        float v[N];
+        Row r;
         Stat a = {-kInf, 0.f, 0.f};
         Teacher<PER> te;
         te.total = 0.f;
         if (w != 0.f) {
-            load_spread<TYPE, N>(x, A.k, v);
             load_entries<PER>(te, A, row);
+            r.load(x, A.k);
             share_out<PER>(te, A);
             load_student<TYPE, PER>(te, x, Part{0, A.k});
-            accumulate<N, false>(v, a, A.c);
+            r.template add<false>(a, A.c);
             a = wave_merge(a, A.c);
         }
         const bool on = w != 0.f && te.total != 0.f, live = on && a.s != 0.f;
@@ -1155,15 +1239,15 @@ __global__ __launch_bounds__(256) void distill_wave_kernel(DistillArgs A) {
                 A.stats[2 * row + 1] = a.s;
             }
         }
-        if (A.dx) {
+        if (!A.dx) continue;
+        if (live) {
             const Ref t_of(a.m, A.c);
-            const float f = live ? w * A.t / a.s : 0.f;
-#pragma unroll
-            for (int j = 0; j < N; ++j)
-                if (lane + 64 * j < A.k)
-                    Elem<TYPE>::store(dx, lane + 64 * j, live ? f * __builtin_amdgcn_exp2f(t_of(v[j])) : 0.f);
+            const float f = w * A.t / a.s;
+            r.write(dx, [&](float v) { return f * __builtin_amdgcn_exp2f(t_of(v)); });
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");      // the row first, then the teacher's classes
-            if (live) fix_gradient<TYPE, PER>(te, a, A, w, dx, Part{0, A.k});
+            fix_gradient<TYPE, PER>(te, a, A, w, dx, Part{0, A.k});
+        } else {
+            for (int i = lane; i < A.k; i += 64) Elem<TYPE>::store(dx, i, 0.f);
         }
     }
 }
@@ -1195,6 +1279,27 @@ int block_threads(const RowsIn& in) {
         else if ((type) == CD_T_BF16) { CALL(CD_T_BF16, __VA_ARGS__); } \
         else { CALL(CD_T_F16, __VA_ARGS__); }                           \
     } while (0)
+
+// CALL(type, row) for the way a wave holds a row of this length
+#define CD_WAVE_ROWS(in, CALL)                                                                     \
+    do {                                                                                           \
+        if ((in).type == CD_T_F32) { CD_WAVE_ROWS_OF(CD_T_F32, (in).k, 4, 8, CALL); }              \
+        else if ((in).type == CD_T_BF16) { CD_WAVE_ROWS_OF(CD_T_BF16, (in).k, 2, 4, CALL); }       \
+        else { CD_WAVE_ROWS_OF(CD_T_F16, (in).k, 2, 4, CALL); }                                    \
+    } while (0)
+#define CD_WAVE_ROWS_OF(TY, k, V1, V2, CALL)                                                       \
+    if ((k) <= 64) { CALL(TY, SpreadRow<TY, 1>); }                                                 \
+    else if ((k) <= 256) { CALL(TY, SpreadRow<TY, 4>); }                                           \
+    else if ((k) <= 512) { CALL(TY, SpreadRow<TY, 8>); }                                           \
+    else if ((k) <= 1024) { CALL(TY, VectorRow<TY, V1>); }                                         \
+    else { CALL(TY, VectorRow<TY, V2>); }
+// ... and of the rows of 16-bit scores beyond kWaveClasses that a wave takes where there are no alternatives to find
+#define CD_WAVE_ROWS_16(in, CALL)                                                                  \
+    do {                                                                                           \
+        if ((in).type == CD_T_BF16) { CALL(CD_T_BF16, VectorRow<CD_T_BF16, 8>); }                  \
+        else { CALL(CD_T_F16, VectorRow<CD_T_F16, 8>); }                                           \
+    } while (0)
+bool wave_row_16(const RowsIn& in) { return in.type != CD_T_F32 && in.k * 2 <= kWaveBytes; }
 
 unsigned thread_grid(int64_t n) { return row_grid((n + 63) / 64); }
 unsigned wave_grid(int64_t n) { return row_grid((n + 3) / 4); }
@@ -1230,9 +1335,9 @@ int launch_log_probs(const RowsIn& in, const int64_t* ids, int top, float* stats
     A.part_keys = reinterpret_cast<uint64_t*>(A.part_stats + in.n * A.parts);
     const dim3 parts((unsigned)in.n, (unsigned)A.parts);
 #define SHORT(TY, K) log_probs_thread_kernel<TY, K><<<thread_grid(in.n), 64, 0, s>>>(A)
-#define WAVE(TY, N)                                                                         \
-    if (entropy) log_probs_wave_kernel<TY, N, true><<<wave_grid(in.n), 256, 0, s>>>(A);     \
-    else log_probs_wave_kernel<TY, N, false><<<wave_grid(in.n), 256, 0, s>>>(A)
+#define WAVE(TY, ...)                                                                               \
+    if (entropy) log_probs_wave_kernel<__VA_ARGS__, true><<<wave_grid(in.n), 256, 0, s>>>(A);       \
+    else log_probs_wave_kernel<__VA_ARGS__, false><<<wave_grid(in.n), 256, 0, s>>>(A)
 #define BLOCK(TY, TH)                                                                       \
     if (entropy) log_probs_block_kernel<TY, TH, true><<<row_grid(in.n), TH, 0, s>>>(A);     \
     else log_probs_block_kernel<TY, TH, false><<<row_grid(in.n), TH, 0, s>>>(A)
@@ -1242,8 +1347,7 @@ int launch_log_probs(const RowsIn& in, const int64_t* ids, int top, float* stats
     log_probs_join_kernel<TY><<<(unsigned)in.n, 64, 0, s>>>(A)
     if (in.k <= 4) CD_BY_TYPE(in.type, SHORT, 4);
     else if (in.k <= kThreadClasses) CD_BY_TYPE(in.type, SHORT, kThreadClasses);
-    else if (in.k <= 256) CD_BY_TYPE(in.type, WAVE, 4);
-    else if (in.k <= kWaveClasses) CD_BY_TYPE(in.type, WAVE, 16);
+    else if (in.k <= kWaveClasses) CD_WAVE_ROWS(in, WAVE);
     else if (A.parts > 1) CD_BY_TYPE(in.type, PARTS, 512);
     else if (block_threads(in) == 256) CD_BY_TYPE(in.type, BLOCK, 256);
     else if (block_threads(in) == 512) CD_BY_TYPE(in.type, BLOCK, 512);
@@ -1263,13 +1367,13 @@ int launch_log_probs_backward(const RowsIn& in, const int64_t* ids, const float*
                                 dx_stride * size, in.k, kLog2e / in.temperature, 1.f / in.temperature, ids, stats,
                                 entropy, g_logp, g_entropy};
 #define SHORT(TY, K) log_probs_grad_thread_kernel<TY, K><<<thread_grid(in.n), 64, 0, s>>>(A)
-#define WAVE(TY, N) log_probs_grad_wave_kernel<TY, N><<<wave_grid(in.n), 256, 0, s>>>(A)
+#define WAVE(TY, ...) log_probs_grad_wave_kernel<__VA_ARGS__, TY><<<wave_grid(in.n), 256, 0, s>>>(A)
     const dim3 grid(row_grid(in.n), grad_parts(in.n, in.k, in.type));
 #define BLOCK(TY, TH) log_probs_grad_kernel<TY, TH><<<grid, TH, 0, s>>>(A)
     if (in.k <= 4) CD_BY_TYPE(in.type, SHORT, 4);
     else if (in.k <= kThreadClasses) CD_BY_TYPE(in.type, SHORT, kThreadClasses);
-    else if (in.k <= 256) CD_BY_TYPE(in.type, WAVE, 4);
-    else if (in.k <= kWaveClasses) CD_BY_TYPE(in.type, WAVE, 16);
+    else if (in.k <= kWaveClasses) CD_WAVE_ROWS(in, WAVE);
+    else if (wave_row_16(in)) CD_WAVE_ROWS_16(in, WAVE);
     else CD_BY_TYPE(in.type, BLOCK, 256);
 #undef SHORT
 #undef WAVE
@@ -1292,17 +1396,17 @@ static DistillArgs distill_args(const RowsIn& in, const TeacherIn& te, float* st
     else if (A.entries <= 128) { TWO; }       \
     else { FOUR; }
 
-// rows of up to kWaveClasses scores, which the gradient alone computes anew; false: longer ones
+// rows that a thread or a wave takes, for which the gradient alone computes everything anew; false: longer ones
 static bool launch_short_distill(const RowsIn& in, const DistillArgs& A, hipStream_t s) {
 #define SHORT(TY, K) distill_thread_kernel<TY, K><<<thread_grid(in.n), 64, 0, s>>>(A)
-#define WAVE(TY, N)                                                                                \
-    PER_LANE((distill_wave_kernel<TY, N, 1><<<wave_grid(in.n), 256, 0, s>>>(A)),                     \
-             (distill_wave_kernel<TY, N, 2><<<wave_grid(in.n), 256, 0, s>>>(A)),                     \
-             (distill_wave_kernel<TY, N, 4><<<wave_grid(in.n), 256, 0, s>>>(A)))
+#define WAVE(TY, ...)                                                                              \
+    PER_LANE((distill_wave_kernel<__VA_ARGS__, TY, 1><<<wave_grid(in.n), 256, 0, s>>>(A)),           \
+             (distill_wave_kernel<__VA_ARGS__, TY, 2><<<wave_grid(in.n), 256, 0, s>>>(A)),           \
+             (distill_wave_kernel<__VA_ARGS__, TY, 4><<<wave_grid(in.n), 256, 0, s>>>(A)))
     if (in.k <= 4 && A.entries <= 16) CD_BY_TYPE(in.type, SHORT, 4);
     else if (in.k <= kThreadClasses && A.entries <= 16) CD_BY_TYPE(in.type, SHORT, kThreadClasses);
-    else if (in.k <= 256) CD_BY_TYPE(in.type, WAVE, 4);
-    else if (in.k <= kWaveClasses) CD_BY_TYPE(in.type, WAVE, 16);
+    else if (in.k <= kWaveClasses) CD_WAVE_ROWS(in, WAVE);
+    else if (wave_row_16(in)) CD_WAVE_ROWS_16(in, WAVE);
     else return false;
 #undef SHORT
 #undef WAVE
