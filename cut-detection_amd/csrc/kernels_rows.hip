@@ -1257,18 +1257,20 @@ unsigned row_grid(int64_t n) { return (unsigned)std::min(n, kMaxGrid); }
 
 int elem_size(int type) { return type == CD_T_F32 ? 4 : 2; }
 
-// Threads of a workgroup that reads a row of more than kWaveClasses scores: many for few rows, since a row's time is then
-// what counts; else as few as keep a few pieces of 64 bytes per thread, so that several rows share a CU and one's reads
-// fill another's waits (4096 rows, 20 alternatives: 8000 x bf16 27 us with 256 threads, 42 with 512, 111 with 1024; 128000 x
-// bf16 263, 217 and 249; 64 rows of 131072 x bf16: 29, 19 and 16).  Where 256 threads, six workgroups to a CU, hold all rows
-// at once and 512, three, would need a second round: 256 (1000 x 50021 f32: 39 us against 44).
+// Threads of a workgroup that reads a row.  With rows enough for every CU, few threads per row: several rows then share a
+// CU, and one's reads fill another's waits (20 alternatives: 30000 x 4000 bf16 98 us with 128 threads, 162 with 256, 301
+// with 512; 20000 x 16000 bf16 174, 159, 209; 8000 x 64000 bf16 327, 243, 215; 4096 x 128000 bf16 263 with 256, 217 with 512, 249
+// with 1024).  With few rows a row's own time counts (200 x 32000 bf16: 20 us with 128, 12.9 with 256, 10 with 512; 64 x
+// 131072 bf16: 29 with 256, 19 with 512, 16 with 1024).  Where 256 threads, six workgroups to a CU, hold all rows at
+// once and 512, three, would need a second round: 256 (1000 x 50021 f32: 39 us against 44).
 int block_threads(const RowsIn& in) {
 #ifdef CD_EXP_ENV
     if (const char* e = std::getenv("CUTDET_X_THREADS")) return std::atoi(e);
 #endif
     const int64_t bytes = (int64_t)in.k * elem_size(in.type);
-    if (bytes <= 32768) return 256;
-    if (in.n <= 256 && bytes > 65536) return 1024;
+    if (bytes <= 16384) return in.n >= 512 ? 128 : 256;
+    if (bytes <= 65536) return in.n >= 512 ? 256 : 512;
+    if (in.n <= 256) return 1024;
     return in.n > 768 && in.n <= 1536 ? 256 : 512;
 }
 
@@ -1349,6 +1351,7 @@ int launch_log_probs(const RowsIn& in, const int64_t* ids, int top, float* stats
     else if (in.k <= kThreadClasses) CD_BY_TYPE(in.type, SHORT, kThreadClasses);
     else if (in.k <= kWaveClasses) CD_WAVE_ROWS(in, WAVE);
     else if (A.parts > 1) CD_BY_TYPE(in.type, PARTS, 512);
+    else if (block_threads(in) == 128) CD_BY_TYPE(in.type, BLOCK, 128);
     else if (block_threads(in) == 256) CD_BY_TYPE(in.type, BLOCK, 256);
     else if (block_threads(in) == 512) CD_BY_TYPE(in.type, BLOCK, 512);
     else CD_BY_TYPE(in.type, BLOCK, 1024);
@@ -1440,6 +1443,7 @@ int launch_distill(const RowsIn& in, const TeacherIn& te, float* stats, float* l
         else if (dx && vectors <= 512 * 8) CD_BY_TYPE(in.type, HELD, 512, 8);
         else if (dx && vectors <= 512 * 16) CD_BY_TYPE(in.type, HELD, 512, 16);
         else if (dx && vectors <= 1024 * 16) CD_BY_TYPE(in.type, HELD, 1024, 16);
+        else if (block_threads(in) == 128) CD_BY_TYPE(in.type, BLOCK, 128);
         else if (block_threads(in) == 256) CD_BY_TYPE(in.type, BLOCK, 256);
         else if (block_threads(in) == 512) CD_BY_TYPE(in.type, BLOCK, 512);
         else CD_BY_TYPE(in.type, BLOCK, 1024);

@@ -283,7 +283,7 @@ class Engine:
     def _grad_rows(self, out, scores):
         """The tensor to write the scores' gradient to."""
         if out is None:
-            return torch.empty(scores.shape, dtype=scores.dtype, device=self.device)
+            return torch.empty(*scores.shape, dtype=scores.dtype, device=self.device)
         self._check_dev(out, "out", scores.dtype)
         n, k = scores.shape
         if tuple(out.shape) != (n, k) or (k > 1 and out.stride(1) != 1) or (n > 1 and out.stride(0) < k):
@@ -297,7 +297,7 @@ class Engine:
     def _workspace(self, scores, top):
         n, k = scores.shape
         size = _rows_workspace(n, k, SCORE_TYPES[scores.dtype], top)
-        return torch.empty((size,), dtype=torch.uint8, device=self.device) if size else None, size
+        return torch.empty(size, dtype=torch.uint8, device=self.device) if size else None, size
 
     def log_probs(self, scores, ids=None, top=0, temperature=1.0, entropy=True):
         """Of every row of scores (f32, bf16 or f16 [n, k]; any row stride), with p = softmax(scores / temperature):
@@ -311,15 +311,15 @@ class Engine:
         if not 0 <= top <= min(64, k):
             raise ValueError(f"top must be in 0..{min(64, k)}, got {top}")
         ids = self._per_row(ids, "ids", torch.int64, n)
-        f32 = dict(dtype=torch.float32, device=self.device)
-        out = {"stats": torch.empty((n, 2), **f32)}
+        dev = self.device
+        out = {"stats": torch.empty(n, 2, dtype=torch.float32, device=dev)}
         if ids is not None:
-            out["logp"] = torch.empty((n,), **f32)
+            out["logp"] = torch.empty(n, dtype=torch.float32, device=dev)
         if entropy:
-            out["entropy"] = torch.empty((n,), **f32)
+            out["entropy"] = torch.empty(n, dtype=torch.float32, device=dev)
         if top:
-            out["top_logp"] = torch.empty((n, top), **f32)
-            out["top_ids"] = torch.empty((n, top), dtype=torch.int64, device=self.device)
+            out["top_logp"] = torch.empty(n, top, dtype=torch.float32, device=dev)
+            out["top_ids"] = torch.empty(n, top, dtype=torch.int64, device=dev)
         if n:
             ws, size = self._workspace(scores, top)
             check(lib.cd_log_probs(self._h, _ptr(scores), SCORE_TYPES[scores.dtype], n, k, self._row_stride(scores),
@@ -375,8 +375,8 @@ class Engine:
         weights = self._per_row(weights, "weights", torch.float32, n)
         if out is not None and not grad:
             raise ValueError("out is for the gradient: pass grad=True")
-        res = {"loss": torch.empty((n,), dtype=torch.float32, device=self.device),
-               "stats": torch.empty((n, 2), dtype=torch.float32, device=self.device)}
+        res = {"loss": torch.empty(n, dtype=torch.float32, device=self.device),
+               "stats": torch.empty(n, 2, dtype=torch.float32, device=self.device)}
         if grad:
             res["grad"] = self._grad_rows(out, scores_in)
         if n:
