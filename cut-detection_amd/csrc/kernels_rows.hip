@@ -12,7 +12,6 @@
 // nothing but -inf has S = 0, log probability -inf everywhere, entropy 0 and gradient 0; a NaN or +inf among the
 // scores makes S, and with it the row's results, NaN.
 #include <algorithm>
-#include <cstdlib>
 
 #include "cd_internal.h"
 
@@ -1264,9 +1263,6 @@ int elem_size(int type) { return type == CD_T_F32 ? 4 : 2; }
 // 131072 bf16: 29 with 256, 19 with 512, 16 with 1024).  Where 256 threads, six workgroups to a CU, hold all rows at
 // once and 512, three, would need a second round: 256 (1000 x 50021 f32: 39 us against 44).
 int block_threads(const RowsIn& in) {
-#ifdef CD_EXP_ENV
-    if (const char* e = std::getenv("CUTDET_X_THREADS")) return std::atoi(e);
-#endif
     const int64_t bytes = (int64_t)in.k * elem_size(in.type);
     if (bytes <= 16384) return in.n >= 512 ? 128 : 256;
     if (bytes <= 65536) return in.n >= 512 ? 256 : 512;

@@ -72,19 +72,38 @@ class ProdNet:
         return self.engine.forward_u8(frames_u8, chan_order=chan_order, net_h=net_h)
 
     # --- training-side reuse ------------------------------------------------------------------
-    def evaluate(self, batches, chan_order=0):
+    def evaluate(self, batches, chan_order=0, per_frame=False, teacher=None):
         """The validation pass of the reference's training script
         (training_scripts/supervised_training.py:177-215) on the fused forward: `batches` yields
         `(x, labels)` pairs or the reference loader's `{"x": ..., "y": ...}` dicts, x being float
         frames [B,3,H,256] or decoded u8 frames [B,H0,W0,3], labels int64 class ids.  Counting and
         the cross-entropy run on the GPU (cd_eval_accumulate).  Returns a dict: `correct`, `total`
         (per class, ints), `accuracy` (per class, correct/total as the script logs it; nan for a
-        class without frames), `loss` (mean cross-entropy per frame), `frames`."""
-        val = Validation(self)
+        class without frames), `loss` (mean cross-entropy per frame), `frames`.
+        `per_frame` adds, under that name, a dict of tensors on the CPU with a row per frame (labelled or
+        not): `logp` (log probability of the label, 0 without one), `entropy`, and `top_ids`, `top_logp`
+        (the two best classes) - the frames to look at again are those with a high entropy or a low logp.
+        `teacher`: another ProdNet on the same GPU (another arithmetic, other weights); adds `divergence`,
+        the mean KL divergence of this net's answers from the teacher's (and its value per frame)."""
+        val = Validation(self, per_frame=per_frame, teacher=teacher)
         for item in batches:
             x, y = (item["x"], item["y"]) if isinstance(item, dict) else item
             val.update(x, y, chan_order=chan_order)
         return val.result()
+
+    def soft_targets(self, x, top=3, chan_order=0):
+        """The classifier as a teacher: (class ids int64 [B, top], log probabilities f32 [B, top]) of the `top`
+        best classes of every frame of x (as in `evaluate`), what cutdet.losses.distill_loss and
+        Engine.distill take to train a student's scores."""
+        eng = self.engine
+        r = eng.log_probs(self._logits(x, chan_order), top=top, entropy=False)
+        return r["top_ids"], r["top_logp"]
+
+    def _logits(self, x, chan_order):
+        x = x.to(self.engine.device)
+        if x.dtype == torch.uint8:
+            return self.engine.forward_u8(x, chan_order=chan_order, want_max=False)
+        return self.engine.forward(x)
 
     def torchscript(self, example=None):
         """What training_scripts/make_torchscript_model.py:25-34 does with the reference's net:
@@ -125,8 +144,11 @@ class Validation:
     """Per-class correct / total counts and the summed cross-entropy of labelled batches, kept on
     the GPU until `result()` (reference training_scripts/supervised_training.py:177-215)."""
 
-    def __init__(self, net, n_classes=3):
+    def __init__(self, net, n_classes=3, per_frame=False, teacher=None):
         self.net = net
+        self.teacher = teacher
+        self.per_frame = bool(per_frame)
+        self.rows = []                # per batch: what `per_frame` and `teacher` ask for, on the GPU
         dev = net.engine.device
         self.correct = torch.zeros((n_classes,), dtype=torch.int64, device=dev)
         self.total = torch.zeros((n_classes,), dtype=torch.int64, device=dev)
@@ -135,18 +157,30 @@ class Validation:
     def update(self, x, labels, chan_order=0):
         eng = self.net.engine
         x = x.to(eng.device)
-        if x.dtype == torch.uint8:
-            logits = eng.forward_u8(x, chan_order=chan_order, want_max=False)
-        else:
-            logits = eng.forward(x)
+        logits = self.net._logits(x, chan_order)
         labels = labels.to(device=eng.device, dtype=torch.int64).reshape(-1)      # the script squeezes [B,1] -> [B]
         eng.eval_accumulate(logits, labels, self.correct, self.total, self.loss_sum)
+        row = {}
+        if self.per_frame:
+            r = eng.log_probs(logits, labels, top=min(2, logits.shape[1]))
+            row = {k: r[k] for k in ("logp", "entropy", "top_ids", "top_logp")}
+        if self.teacher is not None:
+            ids, logp = self.teacher.soft_targets(x, top=logits.shape[1], chan_order=chan_order)
+            row["divergence"] = eng.distill(logits, ids, logp)["loss"]
+        if row:
+            self.rows.append(row)
         return logits
 
     def result(self):
         correct, total = self.correct.cpu().tolist(), self.total.cpu().tolist()
         frames = sum(total)
-        return {"correct": correct, "total": total,
+        extra = {}
+        if self.rows:
+            per = {k: torch.cat([r[k] for r in self.rows]).cpu() for k in self.rows[0]}
+            if "divergence" in per:
+                extra["divergence"] = float(per["divergence"].double().mean())
+            extra["per_frame"] = per
+        return {**extra, "correct": correct, "total": total,
                 "accuracy": [c / t if t else float("nan") for c, t in zip(correct, total)],
                 "loss": float(self.loss_sum.item()) / frames if frames else float("nan"), "frames": frames}
 

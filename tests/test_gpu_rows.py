@@ -496,3 +496,58 @@ def test_a_teachers_alternatives_train_a_student(eng, k):
         ref.check_grad(grad, want[2], want[3], k)
     after = eng.distill(x.detach() - 0.1 * x.grad, t["top_ids"], t["top_logp"])["loss"]
     assert (after < before).all()            # a descent step of a convex function with curvature below 1
+
+
+# ---------------------------------------------------------------------------------------------- the classifier's own paths
+def _clip(eng, n=37):
+    cl = ([0] * 9 + [2] * 4 + [1] * 11 + [0] * 13)[:n]
+    frames = eng.synth_frames(torch.tensor(cl, dtype=torch.uint8, device=eng.device), 180, 320, 5)
+    return frames, torch.tensor(cl, device=eng.device)
+
+
+def test_evaluate_per_frame_and_against_a_teacher(eng):
+    from frameID.net import load_default_net
+    frames, labels_ = _clip(eng)
+    labels_[3] = -1
+    nets = {d: load_default_net(d)[0].to("cuda:0") for d in ("f32", "bf16")}
+    batches = [(frames[:16], labels_[:16]), (frames[16:], labels_[16:])]
+    plain = nets["bf16"].evaluate(batches)
+    assert set(plain) == {"correct", "total", "accuracy", "loss", "frames"}
+    got = nets["bf16"].evaluate(batches, per_frame=True, teacher=nets["f32"])
+    assert all(got[k] == plain[k] for k in plain if k != "loss") and abs(got["loss"] - plain["loss"]) < 1e-9
+    logits = {d: net.classify_frames(frames)[0] for d, net in nets.items()}
+    per = got["per_frame"]
+    want = ref.log_probs64(logits["bf16"], labels_, 1.0, 2)
+    ref.check_logp(per["logp"], want["logp"].cpu(), 3)
+    ref.check_entropy(per["entropy"], want["entropy"].cpu(), 3)
+    assert torch.equal(per["top_ids"], want["top_ids"].cpu())
+    # the mean cross-entropy that eval_accumulate sums is the mean of -logp over the labelled frames
+    assert abs(float(-per["logp"].double().sum()) / got["frames"] - got["loss"]) < 3 * ref.row_error(3) + 1e-6 * got["loss"]
+    lp = ref.log_softmax64(logits["f32"])[0]
+    loss, size, _, _ = ref.distill64(logits["bf16"], torch.arange(3, device="cuda").expand(37, 3), lp)
+    # the teacher's log probabilities are the kernel's: each off by row_error, q by as much
+    d = (per["divergence"].double() - loss.cpu()).abs()
+    assert (d <= 3 * (ref.row_error(3) + 256 * ref.U) * size.cpu()).all()
+    assert abs(got["divergence"] - float(per["divergence"].double().mean())) < 1e-12
+    same = nets["f32"].evaluate(batches, teacher=nets["f32"])
+    assert abs(same["divergence"]) <= 3 * (ref.row_error(3) + 256 * ref.U) * float(size.max())
+
+
+def test_soft_targets_train_a_student_of_the_classifier(eng):
+    """prod_net's answers as targets of a linear student on small frames: gradients through autograd as from the formula."""
+    from cutdet import losses
+    from frameID.net import load_default_net
+    net = load_default_net()[0].to("cuda:0")
+    frames, _ = _clip(eng)
+    ids, logp = net.soft_targets(frames)
+    assert ids.shape == logp.shape == (37, 3) and torch.equal(ids[:, 0], net.classify_frames(frames)[2])
+    feats = frames[:, ::20, ::20].float().reshape(37, -1) / 255
+    g = torch.Generator().manual_seed(1)
+    weight = (torch.randn(3, feats.shape[1], generator=g) * 0.05).cuda().requires_grad_()
+    scores = feats @ weight.t()
+    losses.distill_loss(scores, ids, logp, temperature=2.0).mean().backward()
+    _, _, grad, size = ref.distill64(scores.detach(), ids, logp, None, 2.0)
+    want = (grad.t() / 37) @ feats.double()
+    # 37 products added in 32 bits, each with the scores' gradient off by check_grad's bound
+    bound = ((ref.row_error(3) + 144 * ref.U + 80 * ref.U) * size.t() / 37) @ feats.double()
+    assert ((weight.grad.double() - want).abs() <= bound + 1e-30).all()
