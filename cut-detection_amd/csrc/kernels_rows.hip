@@ -1021,6 +1021,165 @@ __global__ __launch_bounds__(64) void distill_thread_kernel(DistillArgs A) {
     }
 }
 
+// ================================================================================== 16 lanes per row, up to 256 scores
+// Four rows to a wave: reductions stay inside the 16 lanes of a DPP row (rotations, so every lane has the result), and the
+// instructions that a row needs whatever its length are shared by four.  Score i is in lane i % 16.  Alternatives are
+// found one at a time, about 32 instructions each, so many of them are the wave kernel's (100000 x 64 bf16: 4 alternatives
+// 19 us, with a wave per row 60 us; 20 alternatives 52 us and 69 us; 100000 x 200 bf16: 8 alternatives 64 us and 80 us).
+constexpr int kGroupClasses = 256, kGroupEntries = 16;
+inline bool group_tops(int k, int top) { return k <= 64 ? top <= 24 : top <= 8; }
+
+template <int R> __device__ __forceinline__ uint32_t rotated(uint32_t v) {
+    return __builtin_amdgcn_update_dpp(0, v, 0x120 + R, 0xf, 0xf, false);
+}
+template <int R> __device__ __forceinline__ float rotated(float v) { return __uint_as_float(rotated<R>(__float_as_uint(v))); }
+__device__ __forceinline__ float group_sum(float v) {
+    v += rotated<8>(v);
+    v += rotated<4>(v);
+    v += rotated<2>(v);
+    return v + rotated<1>(v);
+}
+__device__ __forceinline__ float group_max(float v) {     // of numbers
+    v = fmaxf(v, rotated<8>(v));
+    v = fmaxf(v, rotated<4>(v));
+    v = fmaxf(v, rotated<2>(v));
+    return fmaxf(v, rotated<1>(v));
+}
+__device__ __forceinline__ uint32_t group_max(uint32_t v) {
+    v = max(v, rotated<8>(v));
+    v = max(v, rotated<4>(v));
+    v = max(v, rotated<2>(v));
+    return max(v, rotated<1>(v));
+}
+__device__ __forceinline__ Stat group_merge(Stat a, float c) {
+    const float m = group_max(a.m);
+    rebase(a, m, c);
+    a.s = group_sum(a.s);
+    a.u = group_sum(a.u);
+    return a;
+}
+template <int TYPE, int N>
+__device__ __forceinline__ void load_group(const char* x, int k, float* v) {
+    const int l = threadIdx.x & 15;
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = l + 16 * j < k ? Elem<TYPE>::load(x, l + 16 * j) : -kInf;
+}
+
+template <int TYPE, int N, bool ENT>
+__global__ __launch_bounds__(256) void log_probs_group_kernel(LogProbsArgs A) {
+    const int l = threadIdx.x & 15;
+    for (int64_t row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4); row < A.n; row += (int64_t)gridDim.x * 16) {
+        const char* x = A.x + row * A.row_bytes;
+        const int id = id_of(A, row);
+        float v[N];
+        load_group<TYPE, N>(x, A.k, v);
+        const float xid = id >= 0 ? Elem<TYPE>::load(x, id) : 0.f;
+        Stat a = {-kInf, 0.f, 0.f};
+        accumulate<N, ENT>(v, a, A.c);
+        a = group_merge(a, A.c);
+        if (l == 0) write_row(A, row, id, xid, a);
+        if (!A.top) continue;
+        uint32_t key[N], used = 0;
+#pragma unroll
+        for (int j = 0; j < N; ++j) key[j] = l + 16 * j < A.k ? score_key(v[j]) : 0;
+        for (int r = 0; r < A.top; ++r) {
+            uint32_t best = 0, at = 0;
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                if (!(used >> j & 1) && key[j] > best) { best = key[j]; at = j; }
+            const uint32_t highest = group_max(best);
+            const uint32_t index = ~group_max(best == highest ? ~(l + 16 * at) : 0u);       // the lowest one
+            if ((index & 15) == l) {
+                used |= 1u << at;
+                write_top(A, row, r, (uint64_t)highest << 32 | ~index, a);
+            }
+        }
+    }
+}
+
+template <int TYPE, int N>
+__global__ __launch_bounds__(256) void log_probs_grad_group_kernel(LogProbsGradArgs A) {
+    const int l = threadIdx.x & 15;
+    for (int64_t row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4); row < A.n; row += (int64_t)gridDim.x * 16) {
+        char* dx = A.dx + row * A.dx_row_bytes;
+        float v[N];
+        load_group<TYPE, N>(A.x + row * A.row_bytes, A.k, v);
+        const float m = A.stats[2 * row], s = A.stats[2 * row + 1];
+        const GradRow g = grad_row(A, row, s);
+        const Ref t_of(m, A.c);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int i = l + 16 * j;
+            if (i < A.k) Elem<TYPE>::store(dx, i, grad_of(t_of(v[j]), g) + (i == g.id ? g.hit : 0.f));
+        }
+    }
+}
+
+template <int TYPE, int N>
+__global__ __launch_bounds__(256) void distill_group_kernel(DistillArgs A) {
+    const int l = threadIdx.x & 15;
+    for (int64_t row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4); row < A.n; row += (int64_t)gridDim.x * 16) {
+        const char* x = A.x + row * A.row_bytes;
+        char* dx = A.dx + row * A.dx_row_bytes;
+        float w = A.weights ? A.weights[row] : 1.f;
+        if (A.g_loss && w != 0.f) w *= A.g_loss[row];
+        float v[N], lq = -kInf, q = 0.f, total = 0.f, sum = 0.f, xj = 0.f;
+        int id = -1;
+        bool first = false;
+        Stat a = {-kInf, 0.f, 0.f};
+        if (w != 0.f) {
+            const int64_t raw = l < A.entries ? A.ids[row * A.entries + l] : -1;
+            load_group<TYPE, N>(x, A.k, v);
+            if (raw >= 0 && raw < A.k) {
+                id = (int)raw;
+                lq = load_any(A.teacher_type, A.teacher, row * A.entries + l);
+                xj = Elem<TYPE>::load(x, id);
+            }
+            accumulate<N, false>(v, a, A.c);
+            a = group_merge(a, A.c);
+            lq = Ref(group_max(lq), A.c)(lq);
+            q = id >= 0 ? __builtin_amdgcn_exp2f(lq) : 0.f;
+            total = group_sum(q);
+            lq -= __builtin_amdgcn_logf(total);
+            q *= 1.f / total;
+            // of a class named more than once the first entry stands for all
+            sum = q;
+            first = id >= 0;
+            auto other = [&](int id2, float q2, uint32_t lane2) {
+                if (id2 == id) {
+                    sum += q2;
+                    if (lane2 < (uint32_t)l) first = false;
+                }
+            };
+            if (A.dx) {
+#define CD_OTHER(R) other((int)rotated<R>((uint32_t)id), rotated<R>(q), rotated<R>((uint32_t)l));
+                CD_OTHER(1) CD_OTHER(2) CD_OTHER(3) CD_OTHER(4) CD_OTHER(5) CD_OTHER(6) CD_OTHER(7) CD_OTHER(8)
+                CD_OTHER(9) CD_OTHER(10) CD_OTHER(11) CD_OTHER(12) CD_OTHER(13) CD_OTHER(14) CD_OTHER(15)
+#undef CD_OTHER
+            }
+        }
+        const bool on = w != 0.f && total != 0.f, live = on && a.s != 0.f;
+        if (A.loss) {
+            const float loss = w * (A.t * A.t) * group_sum(on && id >= 0 ? loss_term(q, lq, xj, a, A.c, A.t) : 0.f);
+            if (l == 0) {
+                A.loss[row] = on ? loss : 0.f;
+                A.stats[2 * row] = a.m;
+                A.stats[2 * row + 1] = a.s;
+            }
+        }
+        if (!A.dx) continue;
+        const Ref t_of(a.m, A.c);
+        const float f = live ? w * A.t / a.s : 0.f;
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            if (l + 16 * j < A.k)
+                Elem<TYPE>::store(dx, l + 16 * j, live ? f * __builtin_amdgcn_exp2f(t_of(v[j])) : 0.f);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");          // the row first, then the teacher's classes
+        if (live && first)
+            Elem<TYPE>::store(dx, id, w * A.t * (__builtin_amdgcn_exp2f(t_of(xj)) * (1.f / a.s) - sum));
+    }
+}
+
 // ================================================================================== one wave per row, up to 4096 scores
 // The row stays in the wave's registers, no barrier, and four rows to a workgroup: 30000 x 2000 bf16 with 20 alternatives
 // takes 61 us so and 152 us with a workgroup per row, 30000 x 4000 loss and gradient 100 us and 183 us.  Beyond 2048
@@ -1300,6 +1459,7 @@ int block_threads(const RowsIn& in) {
 bool wave_row_16(const RowsIn& in) { return in.type != CD_T_F32 && in.k * 2 <= kWaveBytes; }
 
 unsigned thread_grid(int64_t n) { return row_grid((n + 63) / 64); }
+unsigned group_grid(int64_t n) { return row_grid((n + 15) / 16); }
 unsigned wave_grid(int64_t n) { return row_grid((n + 3) / 4); }
 constexpr int64_t kSplitBytes = 128 << 10, kSplitRows = 64;
 
@@ -1339,12 +1499,17 @@ int launch_log_probs(const RowsIn& in, const int64_t* ids, int top, float* stats
 #define BLOCK(TY, TH)                                                                       \
     if (entropy) log_probs_block_kernel<TY, TH, true><<<row_grid(in.n), TH, 0, s>>>(A);     \
     else log_probs_block_kernel<TY, TH, false><<<row_grid(in.n), TH, 0, s>>>(A)
+#define GROUP(TY, N)                                                                                \
+    if (entropy) log_probs_group_kernel<TY, N, true><<<group_grid(in.n), 256, 0, s>>>(A);           \
+    else log_probs_group_kernel<TY, N, false><<<group_grid(in.n), 256, 0, s>>>(A)
 #define PARTS(TY, TH)                                                                       \
     if (entropy) log_probs_part_kernel<TY, TH, true><<<parts, TH, 0, s>>>(A);               \
     else log_probs_part_kernel<TY, TH, false><<<parts, TH, 0, s>>>(A);                      \
     log_probs_join_kernel<TY><<<(unsigned)in.n, 64, 0, s>>>(A)
     if (in.k <= 4) CD_BY_TYPE(in.type, SHORT, 4);
     else if (in.k <= kThreadClasses) CD_BY_TYPE(in.type, SHORT, kThreadClasses);
+    else if (in.k <= 64 && group_tops(in.k, top)) CD_BY_TYPE(in.type, GROUP, 4);
+    else if (in.k <= kGroupClasses && group_tops(in.k, top)) CD_BY_TYPE(in.type, GROUP, 16);
     else if (in.k <= kWaveClasses) CD_WAVE_ROWS(in, WAVE);
     else if (A.parts > 1) CD_BY_TYPE(in.type, PARTS, 512);
     else if (block_threads(in) == 128) CD_BY_TYPE(in.type, BLOCK, 128);
@@ -1353,6 +1518,7 @@ int launch_log_probs(const RowsIn& in, const int64_t* ids, int top, float* stats
     else CD_BY_TYPE(in.type, BLOCK, 1024);
 #undef SHORT
 #undef WAVE
+#undef GROUP
 #undef BLOCK
 #undef PARTS
     CD_HIP(hipGetLastError());
@@ -1366,15 +1532,19 @@ int launch_log_probs_backward(const RowsIn& in, const int64_t* ids, const float*
                                 dx_stride * size, in.k, kLog2e / in.temperature, 1.f / in.temperature, ids, stats,
                                 entropy, g_logp, g_entropy};
 #define SHORT(TY, K) log_probs_grad_thread_kernel<TY, K><<<thread_grid(in.n), 64, 0, s>>>(A)
+#define GROUP(TY, N) log_probs_grad_group_kernel<TY, N><<<group_grid(in.n), 256, 0, s>>>(A)
 #define WAVE(TY, ...) log_probs_grad_wave_kernel<__VA_ARGS__, TY><<<wave_grid(in.n), 256, 0, s>>>(A)
     const dim3 grid(row_grid(in.n), grad_parts(in.n, in.k, in.type));
 #define BLOCK(TY, TH) log_probs_grad_kernel<TY, TH><<<grid, TH, 0, s>>>(A)
     if (in.k <= 4) CD_BY_TYPE(in.type, SHORT, 4);
     else if (in.k <= kThreadClasses) CD_BY_TYPE(in.type, SHORT, kThreadClasses);
+    else if (in.k <= 64) CD_BY_TYPE(in.type, GROUP, 4);
+    else if (in.k <= kGroupClasses) CD_BY_TYPE(in.type, GROUP, 16);
     else if (in.k <= kWaveClasses) CD_WAVE_ROWS(in, WAVE);
     else if (wave_row_16(in)) CD_WAVE_ROWS_16(in, WAVE);
     else CD_BY_TYPE(in.type, BLOCK, 256);
 #undef SHORT
+#undef GROUP
 #undef WAVE
 #undef BLOCK
     CD_HIP(hipGetLastError());
@@ -1398,16 +1568,20 @@ static DistillArgs distill_args(const RowsIn& in, const TeacherIn& te, float* st
 // rows that a thread or a wave takes, for which the gradient alone computes everything anew; false: longer ones
 static bool launch_short_distill(const RowsIn& in, const DistillArgs& A, hipStream_t s) {
 #define SHORT(TY, K) distill_thread_kernel<TY, K><<<thread_grid(in.n), 64, 0, s>>>(A)
+#define GROUP(TY, N) distill_group_kernel<TY, N><<<group_grid(in.n), 256, 0, s>>>(A)
 #define WAVE(TY, ...)                                                                              \
     PER_LANE((distill_wave_kernel<__VA_ARGS__, TY, 1><<<wave_grid(in.n), 256, 0, s>>>(A)),           \
              (distill_wave_kernel<__VA_ARGS__, TY, 2><<<wave_grid(in.n), 256, 0, s>>>(A)),           \
              (distill_wave_kernel<__VA_ARGS__, TY, 4><<<wave_grid(in.n), 256, 0, s>>>(A)))
     if (in.k <= 4 && A.entries <= 16) CD_BY_TYPE(in.type, SHORT, 4);
     else if (in.k <= kThreadClasses && A.entries <= 16) CD_BY_TYPE(in.type, SHORT, kThreadClasses);
+    else if (in.k <= 64 && A.entries <= kGroupEntries) CD_BY_TYPE(in.type, GROUP, 4);
+    else if (in.k <= kGroupClasses && A.entries <= kGroupEntries) CD_BY_TYPE(in.type, GROUP, 16);
     else if (in.k <= kWaveClasses) CD_WAVE_ROWS(in, WAVE);
     else if (wave_row_16(in)) CD_WAVE_ROWS_16(in, WAVE);
     else return false;
 #undef SHORT
+#undef GROUP
 #undef WAVE
     return true;
 }

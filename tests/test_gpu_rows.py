@@ -202,6 +202,50 @@ def test_offsets_beyond_32_bits(eng):
     ref.check_grad(x[-8:], want_g, gsize, k)
 
 
+@pytest.mark.parametrize("n,k", [((4 << 20) + 5, 3), ((4 << 20) + 5, 520), ((16 << 20) + 21, 17), ((1 << 20) + 3, 2050)])
+def test_more_rows_than_a_grid_holds(eng, n, k):
+    """The rows beyond one launch's workgroups are taken by a loop."""
+    x = torch.zeros((n, k), dtype=torch.bfloat16, device="cuda")
+    at = torch.randint(0, n, (40,), generator=torch.Generator().manual_seed(1)).cuda()
+    at[-8:] = torch.arange(n - 8, n, device="cuda")
+    x[at] = rows(40, k, "bf16")
+    some = x[at]
+    ids = torch.zeros(n, dtype=torch.int64, device="cuda")
+    ids[at] = labels(40, k)[:40]
+    got = eng.log_probs(x, ids, top=2)
+    want = ref.log_probs64(some, ids[at], 1.0, 2)
+    ref.check_logp(got["logp"][at], want["logp"], k)
+    ref.check_entropy(got["entropy"][at], want["entropy"], k)
+    assert torch.equal(got["top_ids"][at], want["top_ids"])
+    g = torch.ones(n, device="cuda")
+    grad = eng.log_probs_backward(x, ids, got["stats"], got["entropy"], g, g)
+    ref.check_grad(grad[at], *ref.log_probs_grad64(some, ids[at], g[at], g[at]), k)
+    te = eng.distill(x, got["top_ids"], got["top_logp"], grad=True, out=grad)
+    loss, size, dg, ds = ref.distill64(some, got["top_ids"][at], got["top_logp"][at])
+    ref.check_loss(te["loss"][at], loss, size, k)
+    ref.check_grad(grad[at], dg, ds, k)
+
+
+def test_one_very_long_row(eng):
+    k = (1 << 28) + 5
+    x = torch.empty((1, k), dtype=torch.bfloat16, device="cuda").normal_(generator=torch.Generator("cuda").manual_seed(3))
+    x[0, k - 1], x[0, 0] = 9.0, 9.0
+    ids = torch.tensor([k - 2], device="cuda")
+    got = eng.log_probs(x, ids, top=64)
+    lp, p = ref.log_softmax64(x)
+    ref.check_logp(got["logp"], lp[:, k - 2], k)
+    h = torch.tensor([float(-(p * lp).sum())], dtype=torch.float64, device="cuda")
+    ref.check_entropy(got["entropy"], h, k)
+    order = torch.sort(x[0], descending=True, stable=True)[1][:64]
+    assert torch.equal(got["top_ids"][0], order)
+    at = order[None, :5].contiguous()
+    d = eng.distill(x, at, torch.ones((1, 5), device="cuda"), grad=True)
+    loss = 0.2 * (math.log(0.2) - lp[0, at[0]]).sum()
+    ref.check_loss(d["loss"], loss[None], loss.abs()[None] + 30, k)
+    p[0, at[0]] -= 0.2
+    ref.check_grad(d["grad"], p, p.abs() + 1e-12, k)
+
+
 # ---------------------------------------------------------------------------------------------- gradients
 @pytest.mark.parametrize("dtype", sorted(TYPES))
 @pytest.mark.parametrize("k", [1, 3, 8, 16, 17, 65, 300, 1023, 1025, 5001, 32003, 131075])
