@@ -158,8 +158,9 @@ __device__ __forceinline__ void rebase(Stat& a, float to, float c) {
     a.m = to;
 }
 
+// (returns the largest of x, or NaN)
 template <int N, bool ENT>
-__device__ __forceinline__ void accumulate(const float* x, Stat& a, float c) {
+__device__ __forceinline__ float accumulate(const float* x, Stat& a, float c) {
     float cm = x[0];
 #pragma unroll
     for (int i = 1; i < N; ++i) cm = __builtin_elementwise_maximum(cm, x[i]);
@@ -179,6 +180,7 @@ __device__ __forceinline__ void accumulate(const float* x, Stat& a, float c) {
             if (ENT) a.u = __builtin_fmaf(e, fmaxf(t, -1e4f), a.u);
         }
     }
+    return cm;
 }
 
 __device__ __forceinline__ Stat wave_merge(Stat a, float c) {
@@ -284,8 +286,8 @@ __device__ __forceinline__ void write_top(const LogProbsArgs& A, int64_t row, in
 // The highest classes of a row, from what the pass for the sums leaves behind.  The threads are 64 groups; the K-th
 // largest of the groups' maxima, T, is at most the K-th largest score, since K groups have a score that high.  Only
 // threads whose own maximum reaches T can hold one of the K highest: about K (1 + K / 128) of them for scores in no
-// particular order.  They read their scores again (from the caches), collect those that reach T in a list, and the list
-// is ranked by counting.  Scores equal to T may be very many (a mask): where a wave finds more than kDense threads at T
+// particular order.  They read their scores again (from the caches; most of them only the piece that has their maximum),
+// collect those that reach T in a list, and the list is ranked by counting.  Scores equal to T may be very many (a mask): where a wave finds more than kDense threads at T
 // it leaves them, and the lowest-numbered classes at T are found by a scan in the order of the classes, which then ends
 // early.  A list that overflows all the same (scores laid out against the threads), and NaN, take one scan per class.
 constexpr int kDense = 24;
@@ -295,6 +297,7 @@ template <int THREADS> struct BlockShared {
     uint32_t group[64];
     int count, above, dense, part[kWaves];
     uint8_t lane[kWaves][64];
+    int piece[kWaves][64];
     uint64_t key[kWaves];
     uint64_t list[kList];
 };
@@ -337,15 +340,21 @@ __device__ __forceinline__ Stat block_merge(Stat a, float c, BlockShared<THREADS
     return wave_merge(a, c);
 }
 
+// Where a thread's vectors have their largest score: in the piece of kPiece vectors of that number; `next` is the largest of
+// its other pieces.
+constexpr int kPiece = 4;
+struct Peak { float m, next; int piece; };
+
 // The calling thread's part of the pass over a row.
 template <int TYPE, int THREADS, bool ENT>
-__device__ __forceinline__ Stat block_pass(const char* x, int k, float c) {
+__device__ __forceinline__ Stat block_pass(const char* x, int k, float c, Peak* peak) {
     using E = Elem<TYPE>;
-    constexpr int VE = E::kVec, U = 4;
+    constexpr int VE = E::kVec, U = kPiece;
     const Grid<TYPE> g(x, k);
     const int tid = threadIdx.x;
     const u32x4_any* vec = g.vectors(x);
     Stat a = {-kInf, 0.f, 0.f};
+    *peak = {-kInf, -kInf, 0};
     for (int v0 = 0; v0 < g.nv; v0 += U * THREADS) {
         float xs[U * VE];
 #pragma unroll
@@ -354,7 +363,9 @@ __device__ __forceinline__ Stat block_pass(const char* x, int k, float c) {
             if (v0 + u * THREADS + tid < g.nv) w = vec[v0 + u * THREADS + tid];
             E::unpack(w, xs + u * VE);
         }
-        accumulate<U * VE, ENT>(xs, a, c);
+        const float cm = accumulate<U * VE, ENT>(xs, a, c);
+        peak->next = fmaxf(peak->next, fminf(cm, peak->m));
+        if (cm > peak->m) { peak->m = cm; peak->piece = v0; }
     }
     if (tid < g.extra) {
         const float xt = E::load(x, g.single(tid));
@@ -365,7 +376,7 @@ __device__ __forceinline__ Stat block_pass(const char* x, int k, float c) {
 
 // Calls emit(rank, key) for the K highest of the k scores, every rank once, by any thread.
 template <int TYPE, int THREADS, class Emit>
-__device__ __forceinline__ void block_top(const char* x, int k, int K, float mine, bool nan, BlockShared<THREADS>& sh,
+__device__ __forceinline__ void block_top(const char* x, int k, int K, const Peak& peak, bool nan, BlockShared<THREADS>& sh,
                                           Emit emit) {
     using E = Elem<TYPE>;
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
@@ -380,21 +391,32 @@ __device__ __forceinline__ void block_top(const char* x, int k, int K, float min
                 if (v > xt) atomicAdd(&sh.above, 1);
             }
         };
-        const bool dense = __popcll(__ballot(mine == xt)) > kDense;
-        const uint64_t who = __ballot(dense ? mine > xt : mine >= xt);
+        const bool dense = __popcll(__ballot(peak.m == xt)) > kDense;
         if (dense && lane == 0) sh.dense = 1;
-        if (who >> lane & 1) sh.lane[wave][__popcll(who & ((1ull << lane) - 1))] = lane;
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        const int share = (g.nv + THREADS - 1) / THREADS, items = __popcll(who) * share;
-        for (int it = lane; it < items; it += 64) {
-            const int q = it / share, v = (it - q * share) * THREADS + wave * 64 + sh.lane[wave][q];
-            if (v < g.nv) {
-                float xs[E::kVec];
-                E::unpack(g.vectors(x)[v], xs);
-#pragma unroll
-                for (int i = 0; i < E::kVec; ++i) collect(xs[i], g.head + v * E::kVec + i, !dense);
+        // threads that look into one piece, then threads that look into all of theirs; a lane per vector
+        const bool take = dense ? peak.m > xt : peak.m >= xt, more = dense ? peak.next > xt : peak.next >= xt;
+        auto look = [&](bool mine, int pieces) {
+            const uint64_t who = __ballot(mine);
+            if (mine) {
+                const int at = __popcll(who & ((1ull << lane) - 1));
+                sh.lane[wave][at] = lane;
+                sh.piece[wave][at] = pieces == 1 ? peak.piece : 0;
             }
-        }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            const int share = pieces * kPiece, items = __popcll(who) * share;
+            for (int it = lane; it < items; it += 64) {
+                const int q = it / share, v = sh.piece[wave][q] + (it - q * share) * THREADS + wave * 64 + sh.lane[wave][q];
+                if (v < g.nv) {
+                    float xs[E::kVec];
+                    E::unpack(g.vectors(x)[v], xs);
+#pragma unroll
+                    for (int i = 0; i < E::kVec; ++i) collect(xs[i], g.head + v * E::kVec + i, !dense);
+                }
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        };
+        look(take && !more, 1);
+        if (__any(take && more)) look(take && more, (g.nv + kPiece * THREADS - 1) / (kPiece * THREADS));
         if (tid < g.extra) collect(E::load(x, g.single(tid)), g.single(tid), !dense);
     }
     __syncthreads();
@@ -448,12 +470,13 @@ __global__ __launch_bounds__(THREADS) void log_probs_block_kernel(LogProbsArgs A
     for (int64_t row = blockIdx.x; row < A.n; row += gridDim.x) {
         const char* x = A.x + row * A.row_bytes;
         const int id = id_of(A, row);
-        const Stat own = block_pass<TYPE, THREADS, ENT>(x, A.k, A.c);
+        Peak peak;
+        const Stat own = block_pass<TYPE, THREADS, ENT>(x, A.k, A.c, &peak);
         const float xid = id >= 0 && threadIdx.x == 0 ? Elem<TYPE>::load(x, id) : 0.f;
         const Stat a = block_merge(own, A.c, sh);
         if (threadIdx.x == 0) write_row(A, row, id, xid, a);
         if (A.top)
-            block_top<TYPE>(x, A.k, A.top, own.m, a.s != a.s, sh,
+            block_top<TYPE>(x, A.k, A.top, peak, a.s != a.s, sh,
                             [&](int rank, uint64_t key) { write_top(A, row, rank, key, a); });
         __syncthreads();
     }
@@ -467,13 +490,14 @@ __global__ __launch_bounds__(THREADS) void log_probs_part_kernel(LogProbsArgs A)
     const int64_t row = blockIdx.x, slot = row * A.parts + blockIdx.y;
     const Part p = part_of(A.k, A.parts, blockIdx.y);
     const char* x = A.x + row * A.row_bytes + (int64_t)p.lo * Elem<TYPE>::kSize;
-    const Stat own = block_pass<TYPE, THREADS, ENT>(x, p.hi - p.lo, A.c), a = block_merge(own, A.c, sh);
+    Peak peak;
+    const Stat a = block_merge(block_pass<TYPE, THREADS, ENT>(x, p.hi - p.lo, A.c, &peak), A.c, sh);
     if (threadIdx.x == 0) A.part_stats[slot] = {a.m, a.s, a.u, 0.f};
     if (A.top) {
         uint64_t* keys = A.part_keys + slot * A.top;
         const int have = min(A.top, p.hi - p.lo);
         for (int r = have + threadIdx.x; r < A.top; r += THREADS) keys[r] = 0;
-        if (have) block_top<TYPE>(x, p.hi - p.lo, have, own.m, a.s != a.s, sh,
+        if (have) block_top<TYPE>(x, p.hi - p.lo, have, peak, a.s != a.s, sh,
                                   [&](int rank, uint64_t key) { keys[rank] = key - p.lo; });
     }
 }
@@ -801,7 +825,10 @@ __global__ __launch_bounds__(THREADS) void distill_block_kernel(DistillArgs A) {
         const char* x = A.x + row * A.row_bytes;
         distill_row<TYPE, THREADS, PER>(A, row, all, sh, [] {},
             [&](Teacher<PER>& te) { load_student<TYPE, PER>(te, x, all); },
-            [&] { return block_merge(block_pass<TYPE, THREADS, false>(x, A.k, A.c), A.c, sh); },
+            [&] {
+                Peak peak;
+                return block_merge(block_pass<TYPE, THREADS, false>(x, A.k, A.c, &peak), A.c, sh);
+            },
             [&](float w, const Stat& a) { distill_sweep<TYPE, THREADS>(A, row, all, a, w); });
     }
 }
@@ -819,7 +846,9 @@ __global__ __launch_bounds__(THREADS) void distill_part_kernel(DistillArgs A) {
         const int64_t id = A.ids[row * A.entries + j];
         A.part_x[row * A.entries + j] = id >= 0 && id < A.k ? Elem<TYPE>::load(x, id) : 0.f;
     }
-    const Stat a = block_merge(block_pass<TYPE, THREADS, false>(x + (int64_t)p.lo * Elem<TYPE>::kSize, p.hi - p.lo, A.c), A.c, sh);
+    Peak peak;
+    const Stat a = block_merge(
+        block_pass<TYPE, THREADS, false>(x + (int64_t)p.lo * Elem<TYPE>::kSize, p.hi - p.lo, A.c, &peak), A.c, sh);
     if (threadIdx.x == 0) A.part_stats[row * A.parts + blockIdx.y] = {a.m, a.s, 0.f, 0.f};
 }
 template <int TYPE, int THREADS, int PER>
