@@ -283,13 +283,15 @@ __device__ __forceinline__ void write_top(const LogProbsArgs& A, int64_t row, in
 }
 
 // ================================================================================== one workgroup per row
-// The highest classes of a row, from what the pass for the sums leaves behind.  The threads are 64 groups; the K-th
-// largest of the groups' maxima, T, is at most the K-th largest score, since K groups have a score that high.  Only
-// threads whose own maximum reaches T can hold one of the K highest: about K (1 + K / 128) of them for scores in no
-// particular order.  They read their scores again (from the caches; most of them only the piece that has their maximum),
-// collect those that reach T in a list, and the list is ranked by counting.  Scores equal to T may be very many (a mask): where a wave finds more than kDense threads at T
-// it leaves them, and the lowest-numbered classes at T are found by a scan in the order of the classes, which then ends
-// early.  A list that overflows all the same (scores laid out against the threads), and NaN, take one scan per class.
+// The highest classes of a row, from what the pass for the sums leaves behind.  The threads are 64 groups, lane by lane
+// over the waves (so that high scores side by side fall into different groups); the K-th largest of the groups' maxima, T,
+// is at most the K-th largest score, since K groups have a score that high.  Only threads whose own maximum reaches T can
+// hold one of the K highest: about K (1 + K / 128) of them for scores in no particular order.  They read their scores
+// again (from the caches; most of them only the piece that has their maximum), collect those that reach T in a list, and
+// the list is ranked by counting.  Scores equal to T may be very many (a mask): where a wave finds more than kDense
+// threads at T it leaves them, and the lowest-numbered classes at T are found by a scan in the order of the classes,
+// which then ends early.  A list that overflows all the same (scores laid out against the threads), and NaN, take one
+// scan per class.
 constexpr int kDense = 24;
 template <int THREADS> struct BlockShared {
     static constexpr int kWaves = THREADS / 64, kList = 1024;
@@ -319,20 +321,17 @@ __device__ __forceinline__ uint32_t kth_key(uint32_t key, int K) {
     return t & 0x80000000u ? t : t | ((1u << ZERO_BITS) - 1u);        // (keys of negative scores end in ones)
 }
 
-// The statistics of all threads' parts, the same bits in every thread; one barrier.
-template <int THREADS>
+// The statistics of all threads' parts, the same bits in every thread; one barrier.  TOP: prepares block_top (sh.group is 0
+// before).
+template <bool TOP, int THREADS>
 __device__ __forceinline__ Stat block_merge(Stat a, float c, BlockShared<THREADS>& sh) {
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-    constexpr int G = THREADS / 64;                       // threads of a group
-    float g = a.m;
-    if (G > 1) g = fmaxf(g, dpp<0x111, 0xf>(-kInf, g));
-    if (G > 2) g = fmaxf(g, dpp<0x112, 0xf>(-kInf, g));
-    if (G > 4) g = fmaxf(g, dpp<0x114, 0xf>(-kInf, g));
-    if (G > 8) g = fmaxf(g, dpp<0x118, 0xf>(-kInf, g));
-    if (tid % G == G - 1) sh.group[tid / G] = score_key(g);
+    if (TOP) {
+        atomicMax(&sh.group[lane], score_key(a.m));
+        if (tid == 0) sh.count = sh.above = sh.dense = 0;
+    }
     a = wave_merge(a, c);
     if (lane == 0) { sh.m[wave] = a.m; sh.s[wave] = a.s; sh.u[wave] = a.u; }
-    if (tid == 0) sh.count = sh.above = sh.dense = 0;
     __syncthreads();
     a.m = lane < THREADS / 64 ? sh.m[lane] : -kInf;
     a.s = lane < THREADS / 64 ? sh.s[lane] : 0.f;
@@ -420,6 +419,7 @@ __device__ __forceinline__ void block_top(const char* x, int k, int K, const Pea
         if (tid < g.extra) collect(E::load(x, g.single(tid)), g.single(tid), !dense);
     }
     __syncthreads();
+    if (tid < 64) sh.group[tid] = 0;                      // for the next row, which begins behind a barrier
     const int count = sh.count, above = sh.above, dense = sh.dense;
     if (!nan && count <= sh.kList) {
         for (int e = tid; e < count; e += THREADS) {
@@ -467,13 +467,15 @@ __device__ __forceinline__ void block_top(const char* x, int k, int K, const Pea
 template <int TYPE, int THREADS, bool ENT>
 __global__ __launch_bounds__(THREADS) void log_probs_block_kernel(LogProbsArgs A) {
     __shared__ BlockShared<THREADS> sh;
+    if (threadIdx.x < 64) sh.group[threadIdx.x] = 0;
+    __syncthreads();
     for (int64_t row = blockIdx.x; row < A.n; row += gridDim.x) {
         const char* x = A.x + row * A.row_bytes;
         const int id = id_of(A, row);
         Peak peak;
         const Stat own = block_pass<TYPE, THREADS, ENT>(x, A.k, A.c, &peak);
         const float xid = id >= 0 && threadIdx.x == 0 ? Elem<TYPE>::load(x, id) : 0.f;
-        const Stat a = block_merge(own, A.c, sh);
+        const Stat a = block_merge<true>(own, A.c, sh);
         if (threadIdx.x == 0) write_row(A, row, id, xid, a);
         if (A.top)
             block_top<TYPE>(x, A.k, A.top, peak, a.s != a.s, sh,
@@ -490,8 +492,10 @@ __global__ __launch_bounds__(THREADS) void log_probs_part_kernel(LogProbsArgs A)
     const int64_t row = blockIdx.x, slot = row * A.parts + blockIdx.y;
     const Part p = part_of(A.k, A.parts, blockIdx.y);
     const char* x = A.x + row * A.row_bytes + (int64_t)p.lo * Elem<TYPE>::kSize;
+    if (threadIdx.x < 64) sh.group[threadIdx.x] = 0;
+    __syncthreads();
     Peak peak;
-    const Stat a = block_merge(block_pass<TYPE, THREADS, ENT>(x, p.hi - p.lo, A.c, &peak), A.c, sh);
+    const Stat a = block_merge<true>(block_pass<TYPE, THREADS, ENT>(x, p.hi - p.lo, A.c, &peak), A.c, sh);
     if (threadIdx.x == 0) A.part_stats[slot] = {a.m, a.s, a.u, 0.f};
     if (A.top) {
         uint64_t* keys = A.part_keys + slot * A.top;
@@ -591,13 +595,15 @@ struct LogProbsGradArgs {
     const int64_t* ids;
     const float *stats, *entropy, *g_logp, *g_entropy;
 };
-struct GradRow { float a, b, hit; int id; };    // dx_i = 2^t_i (a + b t_i), plus hit at class id
+// dx_i = 2^t_i (a + b t_i), plus hit at class id; `on` is false where no gradient arrives (the end of a padded batch), or the
+// row has no distribution: 0 then, whatever the scores
+struct GradRow { float a, b, hit; int id; bool on; };
 __device__ __forceinline__ GradRow grad_row(const LogProbsGradArgs& A, int64_t row, float s) {
     const int64_t id = A.ids ? A.ids[row] : -1;
     const bool labelled = id >= 0 && id < A.k;
     const float gl = labelled && A.g_logp ? A.g_logp[row] : 0.f, gh = A.g_entropy ? A.g_entropy[row] : 0.f;
-    GradRow g = {0.f, 0.f, 0.f, -1};
-    if (s == 0.f) return g;
+    GradRow g = {0.f, 0.f, 0.f, -1, s != 0.f && (gl != 0.f || gh != 0.f)};
+    if (!g.on) return g;
     const float inv = A.inv_t / s;
     g.b = -gh * kLn2 * inv;
     g.a = -(gl + gh * ((A.g_entropy ? A.entropy[row] : 0.f) - kLn2 * __builtin_amdgcn_logf(s))) * inv;
@@ -605,6 +611,7 @@ __device__ __forceinline__ GradRow grad_row(const LogProbsGradArgs& A, int64_t r
     g.id = labelled ? (int)id : -1;
     return g;
 }
+// (of a row that is on)
 __device__ __forceinline__ float grad_of(float t, const GradRow& g) {
     return __builtin_amdgcn_exp2f(t) * __builtin_fmaf(g.b, fmaxf(t, -1e4f), g.a);
 }
@@ -622,7 +629,8 @@ __global__ __launch_bounds__(THREADS) void log_probs_grad_kernel(LogProbsGradArg
         const bool here = g.id >= p.lo && g.id < p.hi;
         const float hit = here ? grad_of(t_of(Elem<TYPE>::load(x, g.id - p.lo)), g) + g.hit : 0.f;
         __syncthreads();                                  // (dx may be x)
-        if (t_of.fast) sweep<TYPE, THREADS>(x, dx, p.hi - p.lo, [&](float v) { return grad_of(__builtin_fmaf(v, A.c, -t_of.mc), g); });
+        if (!g.on) clear<TYPE, THREADS>(dx, p.hi - p.lo);
+        else if (t_of.fast) sweep<TYPE, THREADS>(x, dx, p.hi - p.lo, [&](float v) { return grad_of(__builtin_fmaf(v, A.c, -t_of.mc), g); });
         else sweep<TYPE, THREADS>(x, dx, p.hi - p.lo, [&](float v) { return grad_of(t_of(v), g); });
         __syncthreads();                                  // the row first, then its class
         if (threadIdx.x == 0 && here) Elem<TYPE>::store(dx, g.id - p.lo, hit);
@@ -827,7 +835,7 @@ __global__ __launch_bounds__(THREADS) void distill_block_kernel(DistillArgs A) {
             [&](Teacher<PER>& te) { load_student<TYPE, PER>(te, x, all); },
             [&] {
                 Peak peak;
-                return block_merge(block_pass<TYPE, THREADS, false>(x, A.k, A.c, &peak), A.c, sh);
+                return block_merge<false>(block_pass<TYPE, THREADS, false>(x, A.k, A.c, &peak), A.c, sh);
             },
             [&](float w, const Stat& a) { distill_sweep<TYPE, THREADS>(A, row, all, a, w); });
     }
@@ -847,7 +855,7 @@ __global__ __launch_bounds__(THREADS) void distill_part_kernel(DistillArgs A) {
         A.part_x[row * A.entries + j] = id >= 0 && id < A.k ? Elem<TYPE>::load(x, id) : 0.f;
     }
     Peak peak;
-    const Stat a = block_merge(
+    const Stat a = block_merge<false>(
         block_pass<TYPE, THREADS, false>(x + (int64_t)p.lo * Elem<TYPE>::kSize, p.hi - p.lo, A.c, &peak), A.c, sh);
     if (threadIdx.x == 0) A.part_stats[row * A.parts + blockIdx.y] = {a.m, a.s, 0.f, 0.f};
 }
@@ -908,7 +916,7 @@ __global__ __launch_bounds__(THREADS) void distill_held_kernel(DistillArgs A) {
                     accumulate<U * VE, false>(xs, a, A.c);
                 }
                 accumulate<1, false>(&single, a, A.c);
-                return block_merge(a, A.c, sh);
+                return block_merge<false>(a, A.c, sh);
             },
             [&](float weight, const Stat& a) {
                 const Ref t_of(a.m, A.c);
@@ -996,7 +1004,8 @@ __global__ __launch_bounds__(64) void log_probs_grad_thread_kernel(LogProbsGradA
 #pragma unroll
         for (int i = 0; i < K; ++i)
             if (i < A.k)
-                Elem<TYPE>::store(A.dx + row * A.dx_row_bytes, i, grad_of(t_of(v[i]), g) + (i == g.id ? g.hit : 0.f));
+                Elem<TYPE>::store(A.dx + row * A.dx_row_bytes, i,
+                                  g.on ? grad_of(t_of(v[i]), g) + (i == g.id ? g.hit : 0.f) : 0.f);
     }
 }
 
@@ -1139,7 +1148,7 @@ __global__ __launch_bounds__(256) void log_probs_grad_group_kernel(LogProbsGradA
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             const int i = l + 16 * j;
-            if (i < A.k) Elem<TYPE>::store(dx, i, grad_of(t_of(v[j]), g) + (i == g.id ? g.hit : 0.f));
+            if (i < A.k) Elem<TYPE>::store(dx, i, g.on ? grad_of(t_of(v[j]), g) + (i == g.id ? g.hit : 0.f) : 0.f);
         }
     }
 }
@@ -1390,7 +1399,7 @@ __global__ __launch_bounds__(256) void log_probs_grad_wave_kernel(LogProbsGradAr
         const GradRow g = grad_row(A, row, s);
         const Ref t_of(m, A.c);
         const float hit = g.id >= 0 ? grad_of(t_of(r.at(g.id)), g) + g.hit : 0.f;
-        r.write(dx, [&](float v) { return grad_of(t_of(v), g); });
+        r.write(dx, [&](float v) { return g.on ? grad_of(t_of(v), g) : 0.f; });
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");          // the row first, then its class
         if (lane == 0 && g.id >= 0) Elem<TYPE>::store(dx, g.id, hit);
     }
@@ -1485,7 +1494,7 @@ int block_threads(const RowsIn& in) {
         if ((in).type == CD_T_BF16) { CALL(CD_T_BF16, VectorRow<CD_T_BF16, 8>); }                  \
         else { CALL(CD_T_F16, VectorRow<CD_T_F16, 8>); }                                           \
     } while (0)
-bool wave_row_16(const RowsIn& in) { return in.type != CD_T_F32 && in.k * 2 <= kWaveBytes; }
+bool wave_row_16(const RowsIn& in) { return in.type != CD_T_F32 && in.k <= kWaveBytes / 2; }
 
 unsigned thread_grid(int64_t n) { return row_grid((n + 63) / 64); }
 unsigned group_grid(int64_t n) { return row_grid((n + 15) / 16); }

@@ -274,7 +274,8 @@ int cd_log_probs(cd_handle* h, const void* scores, int score_type, int64_t n, in
 
 /* Gradient of sum over rows of grad_logp * logp + grad_entropy * entropy with respect to the scores, rounded once to
  * their type: grad [n][n_classes], grad_stride elements (>= n_classes) between rows.  stats and entropy: of the forward
- * call.  grad_logp (with ids) or grad_entropy (with entropy) may be NULL.  grad may be the scores' own memory with the
+ * call.  grad_logp (with ids) or grad_entropy (with entropy) may be NULL.  A row that no gradient reaches (its id skipped or
+ * its grad_logp 0, and its grad_entropy 0) has gradient 0 whatever its scores.  grad may be the scores' own memory with the
  * scores' stride, and must not overlap with it otherwise. */
 int cd_log_probs_backward(cd_handle* h, const void* scores, int score_type, int64_t n, int n_classes,
                           int64_t row_stride, float temperature, const int64_t* ids, const float* stats,
@@ -284,7 +285,7 @@ int cd_log_probs_backward(cd_handle* h, const void* scores, int score_type, int6
 /* Divergence of every row from a teacher's distribution over `entries` (1 .. 256) classes:
  *   q = softmax(teacher_scores / temperature) over the row's entries, loss = w T^2 sum_j q_j (ln q_j - ln p[id_j])
  * (T^2 keeps the gradient's size independent of the temperature).  teacher_ids i64 [n][entries]: an id outside
- * 0..n_classes-1 marks an unused entry, whose score is not read; a class may be named more than once.  teacher_scores
+ * 0..n_classes-1 marks an unused entry, whose score does not count; a class may be named more than once.  teacher_scores
  * [n][entries] of teacher_type: scores or log probabilities, as cd_log_probs gives them (q does not depend on a constant
  * added to a row).  weights f32 [n] or NULL (all 1): a row of weight 0 is not read, and its loss and gradient are 0, as
  * are those of a row without used entries.  loss f32 [n]; stats f32 [n][2] as in cd_log_probs.

@@ -83,7 +83,12 @@ def log_probs_grad64(x, ids, g_logp, g_entropy, temperature=1.0):
         h = entropy64(lp, p)[:, None]
         grad -= g * torch.where(p == 0, torch.zeros_like(p), p * (lp + h))
         size += g.abs() * torch.where(p == 0, torch.zeros_like(p), p * (lp.abs() + h + math.log(k + 1)))
-    return grad / temperature, size / temperature
+    # a row that no gradient reaches has none, NaN among its scores or not
+    zero = torch.zeros(n, dtype=torch.float64, device=x.device)
+    gl = zero if g_logp is None else torch.where((ids >= 0) & (ids < k), g_logp.double(), 0.0)
+    gh = zero if g_entropy is None else g_entropy.double()
+    off = ((gl == 0) & (gh == 0))[:, None]
+    return torch.where(off, 0.0, grad / temperature), torch.where(off, 0.0, size / temperature)
 
 
 def teacher64(ids, scores, k, temperature):

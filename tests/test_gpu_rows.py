@@ -246,6 +246,25 @@ def test_one_very_long_row(eng):
     ref.check_grad(d["grad"], p, p.abs() + 1e-12, k)
 
 
+def test_the_longest_rows_that_are_allowed(eng):
+    """2^30 classes, where twice the number overflows 32 bits: the last scores count."""
+    k = 1 << 30
+    x = torch.zeros((1, k), dtype=torch.float16, device="cuda")
+    x[0, k - 3:] = 30.0
+    ids = torch.tensor([k - 1], device="cuda")
+    got = eng.log_probs(x, ids, top=4)
+    assert got["top_ids"].tolist() == [[k - 3, k - 2, k - 1, 0]]
+    s = 3 + k * math.exp(-30.0)
+    assert abs(float(got["logp"]) + math.log(s)) <= ref.row_error(k)
+    grad = eng.log_probs_backward(x, ids, got["stats"], None, torch.ones(1, device="cuda"))
+    p = 1 / s
+    assert abs(float(grad[0, k - 1]) - (1 - p)) < 1e-3 and abs(float(grad[0, k - 2]) + p) < 1e-3
+    assert float(grad[0, :k - 3].abs().max()) < 1e-6
+    d = eng.distill(x, ids[:, None], torch.ones((1, 1), device="cuda"), grad=True, out=grad)
+    assert abs(float(d["loss"]) - math.log(s)) <= ref.row_error(k) + 1e-6
+    assert abs(float(grad[0, k - 1]) - (p - 1)) < 1e-3 and abs(float(grad[0, k - 2]) - p) < 1e-3
+
+
 # ---------------------------------------------------------------------------------------------- gradients
 @pytest.mark.parametrize("dtype", sorted(TYPES))
 @pytest.mark.parametrize("k", [1, 3, 8, 16, 17, 65, 300, 1023, 1025, 5001, 32003, 131075])
@@ -265,6 +284,26 @@ def test_log_probs_backward(eng, k, dtype):
         r = eng.log_probs(same, labels(n, k, i), temperature=t)
         got = eng.log_probs_backward(same, labels(n, k, i), r["stats"], r["entropy"], vector(n, 3), vector(n, 4), t, out=same)
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("k", [3, 40, 200, 700, 1500, 4000, 33000, 150001])
+def test_no_gradient_for_the_end_of_a_padded_batch(eng, k, dtype):
+    """Rows without a label, or with upstream gradients of 0, may hold anything."""
+    n = 12
+    x = rows(n, k, dtype)
+    ids = labels(n, k, 2) % k
+    gl, gh = vector(n, 3), vector(n, 4)
+    ids[2:5], gh[2:6], gl[5] = -100, 0.0, 0.0
+    x[2:6] = math.nan
+    x[3, 0], x[4, :] = math.inf, -math.inf
+    r = eng.log_probs(x, ids)
+    got = eng.log_probs_backward(x, ids, r["stats"], r["entropy"], gl, gh)
+    assert not got[2:6].any()
+    ref.check_grad(got, *ref.log_probs_grad64(x, ids, gl, gh), k)
+    got = eng.log_probs_backward(x, ids, r["stats"], None, gl)
+    ref.check_grad(got, *ref.log_probs_grad64(x, ids, gl, None), k)
+    assert not got[2:6].any() and got[0].any()
 
 
 def teacher(n, k, entries, seed=0, dtype="f32"):
