@@ -283,20 +283,20 @@ __device__ __forceinline__ void write_top(const LogProbsArgs& A, int64_t row, in
 }
 
 // ================================================================================== one workgroup per row
-// The highest classes of a row, from what the pass for the sums leaves behind.  The threads are 64 groups, lane by lane
-// over the waves (so that high scores side by side fall into different groups); the K-th largest of the groups' maxima, T,
-// is at most the K-th largest score, since K groups have a score that high.  Only threads whose own maximum reaches T can
-// hold one of the K highest: about K (1 + K / 128) of them for scores in no particular order.  They read their scores
-// again (from the caches; most of them only the piece that has their maximum), collect those that reach T in a list, and
-// the list is ranked by counting.  Scores equal to T may be very many (a mask): where a wave finds more than kDense
-// threads at T it leaves them, and the lowest-numbered classes at T are found by a scan in the order of the classes,
-// which then ends early.  A list that overflows all the same (scores laid out against the threads), and NaN, take one
-// scan per class.
-constexpr int kDense = 24;
+// The highest classes of a row, from what the pass for the sums leaves behind.  The threads are 64 groups (256 for more
+// than kFewTops alternatives), lane by lane over the waves, so that high scores side by side fall into different groups;
+// the K-th largest of the groups' maxima, T, is at most the K-th largest score, since K groups have a score that high.
+// Only threads whose own maximum reaches T can hold one of the K highest: about K (1 + K / 128), with 256 groups
+// K (1 + K / 512), for scores in no particular order.  They read their scores again (from the caches; most of them only the
+// piece that has their maximum), collect those that reach T in a list, and the list is ranked by counting.  Scores equal
+// to T may be very many (a mask): where a wave finds more than kDense threads at T it leaves them, and the
+// lowest-numbered classes at T are found by a scan in the order of the classes, which then ends early.  A list that
+// overflows all the same (scores laid out against the threads), and NaN, take one scan per class.
+constexpr int kDense = 24, kFewTops = 24;
 template <int THREADS> struct BlockShared {
     static constexpr int kWaves = THREADS / 64, kList = 1024;
     float m[kWaves], s[kWaves], u[kWaves], total;
-    uint32_t group[64];
+    uint32_t group[256];
     int count, above, dense, part[kWaves];
     uint8_t lane[kWaves][64];
     int piece[kWaves][64];
@@ -304,30 +304,36 @@ template <int THREADS> struct BlockShared {
     uint64_t list[kList];
 };
 
-// the K-th largest of 64 lanes' keys
-template <int ZERO_BITS>
-__device__ __forceinline__ uint32_t kth_key(uint32_t key, int K) {
-    uint32_t t = 0;
-    const uint32_t part = key >> ZERO_BITS;
+// the K-th largest of 64 lanes' keys, N to a lane
+template <int ZERO_BITS, int N>
+__device__ __forceinline__ uint32_t kth_key(const uint32_t (&key)[N], int K) {
+    uint32_t t = 0, part[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) part[i] = key[i] >> ZERO_BITS;
+    auto reach = [&](uint32_t v) {
+        int c = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) c += __popcll(__ballot(part[i] >= v));
+        return c >= K;
+    };
     constexpr int kBits = 32 - ZERO_BITS;
-    if (kBits & 1 && __popcll(__ballot(part >> (kBits - 1) != 0)) >= K) t = 1u << (kBits - 1);
+    if (kBits & 1 && reach(1u << (kBits - 1))) t = 1u << (kBits - 1);
 #pragma unroll
     for (int b = kBits / 2 * 2 - 2; b >= 0; b -= 2) {     // two bits a step: three counts that do not wait for one another
-        const int c1 = __popcll(__ballot(part >= (t | 1u << b))), c2 = __popcll(__ballot(part >= (t | 2u << b))),
-                  c3 = __popcll(__ballot(part >= (t | 3u << b)));
-        t |= (c3 >= K ? 3u : c2 >= K ? 2u : c1 >= K ? 1u : 0u) << b;
+        const bool r1 = reach(t | 1u << b), r2 = reach(t | 2u << b), r3 = reach(t | 3u << b);
+        t |= (r3 ? 3u : r2 ? 2u : r1 ? 1u : 0u) << b;
     }
     t <<= ZERO_BITS;
     return t & 0x80000000u ? t : t | ((1u << ZERO_BITS) - 1u);        // (keys of negative scores end in ones)
 }
 
-// The statistics of all threads' parts, the same bits in every thread; one barrier.  TOP: prepares block_top (sh.group is 0
-// before).
+// The statistics of all threads' parts, the same bits in every thread; one barrier.  TOP: prepares block_top for that many
+// alternatives (sh.group is 0 before).
 template <bool TOP, int THREADS>
-__device__ __forceinline__ Stat block_merge(Stat a, float c, BlockShared<THREADS>& sh) {
+__device__ __forceinline__ Stat block_merge(Stat a, float c, BlockShared<THREADS>& sh, int top = 0) {
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     if (TOP) {
-        atomicMax(&sh.group[lane], score_key(a.m));
+        atomicMax(&sh.group[top > kFewTops ? tid & 255 : lane], score_key(a.m));
         if (tid == 0) sh.count = sh.above = sh.dense = 0;
     }
     a = wave_merge(a, c);
@@ -380,7 +386,14 @@ __device__ __forceinline__ void block_top(const char* x, int k, int K, const Pea
     using E = Elem<TYPE>;
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     const Grid<TYPE> g(x, k);
-    const uint32_t T = kth_key<E::kZeroBits>(sh.group[lane], K);
+    uint32_t T;
+    if (K > kFewTops) {
+        const uint32_t key[4] = {sh.group[lane], sh.group[lane + 64], sh.group[lane + 128], sh.group[lane + 192]};
+        T = kth_key<E::kZeroBits, 4>(key, K);
+    } else {
+        const uint32_t key[1] = {sh.group[lane]};
+        T = kth_key<E::kZeroBits, 1>(key, K);
+    }
     if (!nan) {
         const float xt = key_score(T);
         auto collect = [&](float v, uint32_t i, bool ties) {
@@ -419,7 +432,7 @@ __device__ __forceinline__ void block_top(const char* x, int k, int K, const Pea
         if (tid < g.extra) collect(E::load(x, g.single(tid)), g.single(tid), !dense);
     }
     __syncthreads();
-    if (tid < 64) sh.group[tid] = 0;                      // for the next row, which begins behind a barrier
+    for (int i = tid; i < 256; i += THREADS) sh.group[i] = 0;     // for the next row, which begins behind a barrier
     const int count = sh.count, above = sh.above, dense = sh.dense;
     if (!nan && count <= sh.kList) {
         for (int e = tid; e < count; e += THREADS) {
@@ -467,7 +480,7 @@ __device__ __forceinline__ void block_top(const char* x, int k, int K, const Pea
 template <int TYPE, int THREADS, bool ENT>
 __global__ __launch_bounds__(THREADS) void log_probs_block_kernel(LogProbsArgs A) {
     __shared__ BlockShared<THREADS> sh;
-    if (threadIdx.x < 64) sh.group[threadIdx.x] = 0;
+    for (int i = threadIdx.x; i < 256; i += THREADS) sh.group[i] = 0;
     __syncthreads();
     for (int64_t row = blockIdx.x; row < A.n; row += gridDim.x) {
         const char* x = A.x + row * A.row_bytes;
@@ -475,7 +488,7 @@ __global__ __launch_bounds__(THREADS) void log_probs_block_kernel(LogProbsArgs A
         Peak peak;
         const Stat own = block_pass<TYPE, THREADS, ENT>(x, A.k, A.c, &peak);
         const float xid = id >= 0 && threadIdx.x == 0 ? Elem<TYPE>::load(x, id) : 0.f;
-        const Stat a = block_merge<true>(own, A.c, sh);
+        const Stat a = block_merge<true>(own, A.c, sh, A.top);
         if (threadIdx.x == 0) write_row(A, row, id, xid, a);
         if (A.top)
             block_top<TYPE>(x, A.k, A.top, peak, a.s != a.s, sh,
@@ -491,15 +504,15 @@ __global__ __launch_bounds__(THREADS) void log_probs_part_kernel(LogProbsArgs A)
     __shared__ BlockShared<THREADS> sh;
     const int64_t row = blockIdx.x, slot = row * A.parts + blockIdx.y;
     const Part p = part_of(A.k, A.parts, blockIdx.y);
+    const int have = min(A.top, p.hi - p.lo);
     const char* x = A.x + row * A.row_bytes + (int64_t)p.lo * Elem<TYPE>::kSize;
-    if (threadIdx.x < 64) sh.group[threadIdx.x] = 0;
+    for (int i = threadIdx.x; i < 256; i += THREADS) sh.group[i] = 0;
     __syncthreads();
     Peak peak;
-    const Stat a = block_merge<true>(block_pass<TYPE, THREADS, ENT>(x, p.hi - p.lo, A.c, &peak), A.c, sh);
+    const Stat a = block_merge<true>(block_pass<TYPE, THREADS, ENT>(x, p.hi - p.lo, A.c, &peak), A.c, sh, have);
     if (threadIdx.x == 0) A.part_stats[slot] = {a.m, a.s, a.u, 0.f};
     if (A.top) {
         uint64_t* keys = A.part_keys + slot * A.top;
-        const int have = min(A.top, p.hi - p.lo);
         for (int r = have + threadIdx.x; r < A.top; r += THREADS) keys[r] = 0;
         if (have) block_top<TYPE>(x, p.hi - p.lo, have, peak, a.s != a.s, sh,
                                   [&](int rank, uint64_t key) { keys[rank] = key - p.lo; });
@@ -1323,7 +1336,8 @@ __device__ __forceinline__ void wave_top(Row& r, int K, float mine, bool nan, ui
     int count = 0;
     r.pin();
     if (!nan) {
-        const float t = key_score(kth_key<0>(score_key(mine), K));
+        const uint32_t high[1] = {score_key(mine)};
+        const float t = key_score(kth_key<0, 1>(high, K));
 #pragma unroll
         for (int j = 0; j < Row::kCount; ++j) {
             const bool take = r.value(j) >= t && r.valid(j);
