@@ -304,7 +304,8 @@ class Engine:
         `logp` [n], the log probability of class ids[row] (int64 [n]; 0 where the id is outside 0..k-1);
         `entropy` [n]; `top_logp`, `top_ids` [n, top], the classes with the highest scores (at most 64, equal scores
         in the order of their index); `stats` [n, 2] for log_probs_backward.  A dict of float32 (ids: int64)
-        tensors, without what was not asked for.  See cd_log_probs for -inf, NaN and rows without a distribution."""
+        tensors, without what was not asked for; no autograd (cutdet.losses has it).  See cd_log_probs for -inf, NaN and
+        rows without a distribution."""
         scores = self._score_rows(scores)
         n, k = scores.shape
         top = int(top)
