@@ -538,11 +538,13 @@ __global__ __launch_bounds__(64) void log_probs_join_kernel(LogProbsArgs A) {
     const uint64_t* keys = A.part_keys + row * A.parts * A.top;
     const int heads = 64 / A.parts, q = lane / heads, r = lane - q * heads;
     const uint64_t mine = q < A.parts && r < A.top ? keys[q * A.top + r] : 0;
-    uint64_t t = 0;
-    for (int b = 63; b >= 0; --b) {
-        const uint64_t up = t | 1ull << b;
-        if (__popcll(__ballot(mine >= up)) >= A.top) t = up;
-    }
+    const uint32_t high[1] = {(uint32_t)(mine >> 32)};
+    uint64_t t = (uint64_t)kth_key<0, 1>(high, A.top) << 32;
+    if (__popcll(__ballot(mine >= t)) >= A.top + 16)      // many equal scores: the classes count as well
+        for (int b = 31; b >= 0; --b) {
+            const uint64_t up = t | 1ull << b;
+            if (__popcll(__ballot(mine >= up)) >= A.top) t = up;
+        }
     int count = 0;
     for (int e = lane; e - lane < A.parts * A.top; e += 64) {
         const uint64_t key = e < A.parts * A.top ? keys[e] : 0;

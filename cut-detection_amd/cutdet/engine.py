@@ -63,6 +63,9 @@ class Engine:
         self.device = torch.device("cuda", index)
         self._blob = bytes(blob)
         self._h = C.c_void_p(0)
+        # new_empty of a tensor at hand: less host time per output than torch.empty(..., dtype, device)
+        self._new_f32 = torch.empty(0, dtype=torch.float32, device=self.device).new_empty
+        self._new_i64 = torch.empty(0, dtype=torch.int64, device=self.device).new_empty
         check(lib.cd_create(C.byref(self._h), self._blob, len(self._blob), index, _lib.DTYPES[dtype]))
 
     def close(self):
@@ -267,8 +270,8 @@ class Engine:
             raise RuntimeError(f"scores must be a tensor on {self.device} (got {getattr(scores, 'device', type(scores))})")
         if scores.dtype not in SCORE_TYPES:
             raise TypeError(f"scores must be float32, bfloat16 or float16, got {scores.dtype}")
-        if scores.dim() != 2 or scores.shape[1] < 1:
-            raise ValueError("scores must be [n, k]")
+        if scores.dim() != 2 or not 1 <= scores.shape[1] <= 1 << 30:
+            raise ValueError(f"scores must be [n, k] with 1 to 2^30 classes, got {tuple(scores.shape)}")
         return scores if scores.shape[1] == 1 or scores.stride(1) == 1 else scores.contiguous()
 
     def _per_row(self, t, name, dtype, n, *more):
@@ -283,7 +286,7 @@ class Engine:
     def _grad_rows(self, out, scores):
         """The tensor to write the scores' gradient to."""
         if out is None:
-            return torch.empty(*scores.shape, dtype=scores.dtype, device=self.device)
+            return scores.new_empty(scores.shape)
         self._check_dev(out, "out", scores.dtype)
         n, k = scores.shape
         if tuple(out.shape) != (n, k) or (k > 1 and out.stride(1) != 1) or (n > 1 and out.stride(0) < k):
@@ -312,15 +315,15 @@ class Engine:
         if not 0 <= top <= min(64, k):
             raise ValueError(f"top must be in 0..{min(64, k)}, got {top}")
         ids = self._per_row(ids, "ids", torch.int64, n)
-        dev = self.device
-        out = {"stats": torch.empty(n, 2, dtype=torch.float32, device=dev)}
+        new = self._new_f32
+        out = {"stats": new(n, 2)}
         if ids is not None:
-            out["logp"] = torch.empty(n, dtype=torch.float32, device=dev)
+            out["logp"] = new(n)
         if entropy:
-            out["entropy"] = torch.empty(n, dtype=torch.float32, device=dev)
+            out["entropy"] = new(n)
         if top:
-            out["top_logp"] = torch.empty(n, top, dtype=torch.float32, device=dev)
-            out["top_ids"] = torch.empty(n, top, dtype=torch.int64, device=dev)
+            out["top_logp"] = new(n, top)
+            out["top_ids"] = self._new_i64(n, top)
         if n:
             ws, size = self._workspace(scores, top)
             check(lib.cd_log_probs(self._h, _ptr(scores), SCORE_TYPES[scores.dtype], n, k, self._row_stride(scores),
@@ -376,8 +379,7 @@ class Engine:
         weights = self._per_row(weights, "weights", torch.float32, n)
         if out is not None and not grad:
             raise ValueError("out is for the gradient: pass grad=True")
-        res = {"loss": torch.empty(n, dtype=torch.float32, device=self.device),
-               "stats": torch.empty(n, 2, dtype=torch.float32, device=self.device)}
+        res = {"loss": self._new_f32(n), "stats": self._new_f32(n, 2)}
         if grad:
             res["grad"] = self._grad_rows(out, scores_in)
         if n:

@@ -110,6 +110,7 @@ IDS = torch.zeros(4, 2, dtype=torch.int64)
     (lambda e: e.log_probs(X.double()), TypeError),
     (lambda e: e.log_probs(X[0]), ValueError),
     (lambda e: e.log_probs(X[:, :0]), ValueError),
+    (lambda e: e.log_probs(torch.zeros(1).expand(1, (1 << 32) + 5)), ValueError),      # 5 in 32 bits
     (lambda e: e.log_probs(X, top=7), ValueError),
     (lambda e: e.log_probs(X, top=-1), ValueError),
     (lambda e: e.log_probs(torch.zeros(1, 100), top=65), ValueError),
