@@ -497,8 +497,8 @@ __global__ __launch_bounds__(THREADS) void log_probs_block_kernel(LogProbsArgs A
     }
 }
 
-// Few, long rows: several workgroups per row leave their statistics and highest classes in the workspace, and one wave
-// per row joins them.
+// Few, long rows: several workgroups per row leave their statistics and highest classes in the workspace, and one
+// workgroup per row joins them.
 template <int TYPE, int THREADS, bool ENT>
 __global__ __launch_bounds__(THREADS) void log_probs_part_kernel(LogProbsArgs A) {
     __shared__ BlockShared<THREADS> sh;
@@ -524,37 +524,52 @@ __device__ __forceinline__ Stat join_stats(const float4* part, int parts, float 
     if (lane < parts) { const float4 v = part[lane]; a = {v.x, v.y, v.z}; }
     return wave_merge(a, c);
 }
+// A bound as in block_top, from the first keys of every part, 64 N in all.
+template <int N>
+__device__ __forceinline__ uint64_t join_bound(const uint64_t* keys, int parts, int top) {
+    const int lane = threadIdx.x & 63, heads = 64 * N / parts;
+    uint64_t mine[N];
+    uint32_t high[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const int q = (lane + 64 * j) / heads, r = lane + 64 * j - q * heads;
+        mine[j] = q < parts && r < top ? keys[q * top + r] : 0;
+        high[j] = (uint32_t)(mine[j] >> 32);
+    }
+    auto reach = [&](uint64_t v) {
+        int c = 0;
+#pragma unroll
+        for (int j = 0; j < N; ++j) c += __popcll(__ballot(mine[j] >= v));
+        return c;
+    };
+    uint64_t t = (uint64_t)kth_key<0, N>(high, top) << 32;
+    if (reach(t) >= top + 16)                             // many equal scores: the classes count as well
+        for (int b = 31; b >= 0; --b)
+            if (reach(t | 1ull << b) >= top) t |= 1ull << b;
+    return t;
+}
 template <int TYPE>
-__global__ __launch_bounds__(64) void log_probs_join_kernel(LogProbsArgs A) {
+__global__ __launch_bounds__(256) void log_probs_join_kernel(LogProbsArgs A) {
     __shared__ uint64_t list[64 * kMaxTop];
-    const int lane = threadIdx.x;
+    __shared__ int count;
+    const int tid = threadIdx.x;
     const int64_t row = blockIdx.x;
     const int id = id_of(A, row);
     const float xid = id >= 0 ? Elem<TYPE>::load(A.x + row * A.row_bytes, id) : 0.f;
     const Stat a = join_stats(A.part_stats + row * A.parts, A.parts, A.c);
-    if (lane == 0) write_row(A, row, id, xid, a);
+    if (tid == 0) write_row(A, row, id, xid, a);
     if (!A.top) return;
-    // of every part the first 64 / parts: 64 keys, whose K-th largest is a bound as in block_top
+    if (tid == 0) count = 0;
+    __syncthreads();
     const uint64_t* keys = A.part_keys + row * A.parts * A.top;
-    const int heads = 64 / A.parts, q = lane / heads, r = lane - q * heads;
-    const uint64_t mine = q < A.parts && r < A.top ? keys[q * A.top + r] : 0;
-    const uint32_t high[1] = {(uint32_t)(mine >> 32)};
-    uint64_t t = (uint64_t)kth_key<0, 1>(high, A.top) << 32;
-    if (__popcll(__ballot(mine >= t)) >= A.top + 16)      // many equal scores: the classes count as well
-        for (int b = 31; b >= 0; --b) {
-            const uint64_t up = t | 1ull << b;
-            if (__popcll(__ballot(mine >= up)) >= A.top) t = up;
-        }
-    int count = 0;
-    for (int e = lane; e - lane < A.parts * A.top; e += 64) {
-        const uint64_t key = e < A.parts * A.top ? keys[e] : 0;
-        const bool take = key != 0 && key >= t;
-        const uint64_t taken = __ballot(take);
-        if (take) list[count + __popcll(taken & ((1ull << lane) - 1))] = key;
-        count += __popcll(taken);
+    const uint64_t t = A.top > kFewTops ? join_bound<4>(keys, A.parts, A.top) : join_bound<1>(keys, A.parts, A.top);
+#pragma unroll 4
+    for (int e = tid; e < A.parts * A.top; e += 256) {
+        const uint64_t key = keys[e];
+        if (key != 0 && key >= t) list[atomicAdd(&count, 1)] = key;       // (in any order: they are ranked)
     }
     __syncthreads();
-    for (int e = lane; e < count; e += 64) {
+    for (int e = tid; e < count; e += 256) {
         const uint64_t key = list[e];
         int rank = 0;
 #pragma unroll 8
@@ -1562,7 +1577,7 @@ int launch_log_probs(const RowsIn& in, const int64_t* ids, int top, float* stats
 #define PARTS(TY, TH)                                                                       \
     if (entropy) log_probs_part_kernel<TY, TH, true><<<parts, TH, 0, s>>>(A);               \
     else log_probs_part_kernel<TY, TH, false><<<parts, TH, 0, s>>>(A);                      \
-    log_probs_join_kernel<TY><<<(unsigned)in.n, 64, 0, s>>>(A)
+    log_probs_join_kernel<TY><<<(unsigned)in.n, 256, 0, s>>>(A)
     if (in.k <= 4) CD_BY_TYPE(in.type, SHORT, 4);
     else if (in.k <= kThreadClasses) CD_BY_TYPE(in.type, SHORT, kThreadClasses);
     else if (in.k <= 64 && group_tops(in.k, top)) CD_BY_TYPE(in.type, GROUP, 4);
