@@ -1506,20 +1506,22 @@ int block_threads(const RowsIn& in) {
         else { CALL(CD_T_F16, __VA_ARGS__); }                           \
     } while (0)
 
-// CALL(type, row) for the way a wave holds a row of this length
+// CALL(type, row) for the way a wave holds a row of up to kGroupClasses scores, ...
+#define CD_WAVE_ROWS_SHORT(in, CALL)                                                               \
+    do {                                                                                           \
+        if ((in).k <= 64) { CD_BY_TYPE((in).type, CD_SPREAD, 1, CALL); }                           \
+        else { CD_BY_TYPE((in).type, CD_SPREAD, 4, CALL); }                                        \
+    } while (0)
+#define CD_SPREAD(TY, N, CALL) CALL(TY, SpreadRow<TY, N>)
+// ... of up to kWaveClasses, ...
 #define CD_WAVE_ROWS(in, CALL)                                                                     \
     do {                                                                                           \
-        if ((in).type == CD_T_F32) { CD_WAVE_ROWS_OF(CD_T_F32, (in).k, 4, 8, CALL); }              \
-        else if ((in).type == CD_T_BF16) { CD_WAVE_ROWS_OF(CD_T_BF16, (in).k, 2, 4, CALL); }       \
-        else { CD_WAVE_ROWS_OF(CD_T_F16, (in).k, 2, 4, CALL); }                                    \
+        if ((in).k <= 512) { CD_BY_TYPE((in).type, CD_SPREAD, 8, CALL); }                          \
+        else if ((in).k <= 1024) { CD_BY_TYPE((in).type, CD_VECTORS, 1, CALL); }                   \
+        else { CD_BY_TYPE((in).type, CD_VECTORS, 2, CALL); }                                       \
     } while (0)
-#define CD_WAVE_ROWS_OF(TY, k, V1, V2, CALL)                                                       \
-    if ((k) <= 64) { CALL(TY, SpreadRow<TY, 1>); }                                                 \
-    else if ((k) <= 256) { CALL(TY, SpreadRow<TY, 4>); }                                           \
-    else if ((k) <= 512) { CALL(TY, SpreadRow<TY, 8>); }                                           \
-    else if ((k) <= 1024) { CALL(TY, VectorRow<TY, V1>); }                                         \
-    else { CALL(TY, VectorRow<TY, V2>); }
-// ... and of the rows of 16-bit scores beyond kWaveClasses that a wave takes where there are no alternatives to find
+#define CD_VECTORS(TY, KILO, CALL) CALL(TY, VectorRow<TY, 16 / Elem<TY>::kVec * KILO>)
+// ... and of the 16-bit scores beyond that a wave takes where there are no alternatives to find
 #define CD_WAVE_ROWS_16(in, CALL)                                                                  \
     do {                                                                                           \
         if ((in).type == CD_T_BF16) { CALL(CD_T_BF16, VectorRow<CD_T_BF16, 8>); }                  \
@@ -1582,6 +1584,7 @@ int launch_log_probs(const RowsIn& in, const int64_t* ids, int top, float* stats
     else if (in.k <= kThreadClasses) CD_BY_TYPE(in.type, SHORT, kThreadClasses);
     else if (in.k <= 64 && group_tops(in.k, top)) CD_BY_TYPE(in.type, GROUP, 4);
     else if (in.k <= kGroupClasses && group_tops(in.k, top)) CD_BY_TYPE(in.type, GROUP, 16);
+    else if (in.k <= kGroupClasses) CD_WAVE_ROWS_SHORT(in, WAVE);
     else if (in.k <= kWaveClasses) CD_WAVE_ROWS(in, WAVE);
     else if (A.parts > 1) CD_BY_TYPE(in.type, PARTS, 512);
     else if (block_threads(in) == 128) CD_BY_TYPE(in.type, BLOCK, 128);
@@ -1649,6 +1652,7 @@ static bool launch_short_distill(const RowsIn& in, const DistillArgs& A, hipStre
     else if (in.k <= kThreadClasses && A.entries <= 16) CD_BY_TYPE(in.type, SHORT, kThreadClasses);
     else if (in.k <= 64 && A.entries <= kGroupEntries) CD_BY_TYPE(in.type, GROUP, 4);
     else if (in.k <= kGroupClasses && A.entries <= kGroupEntries) CD_BY_TYPE(in.type, GROUP, 16);
+    else if (in.k <= kGroupClasses) CD_WAVE_ROWS_SHORT(in, WAVE);
     else if (in.k <= kWaveClasses) CD_WAVE_ROWS(in, WAVE);
     else if (wave_row_16(in)) CD_WAVE_ROWS_16(in, WAVE);
     else return false;
