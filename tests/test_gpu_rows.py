@@ -558,6 +558,21 @@ def test_captured_gradients_of_a_leaf_are_refused(eng):
     with pytest.raises(RuntimeError, match="leaf"):
         with torch.cuda.graph(torch.cuda.CUDAGraph()):
             losses.log_probs(x, ids)
+    at, te = teacher(4, 20, 3)
+    with pytest.raises(RuntimeError, match="captured"):                # not a leaf itself, but made of one
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            losses.distill_loss(x * 2, at, te)
+    with torch.no_grad():                                              # nothing to differentiate: may be captured
+        want = losses.distill_loss(x, at, te)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = losses.distill_loss(x, at, te)
+    for _ in range(3):
+        got.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
     assert torch.isfinite(losses.log_probs(x, ids)[1]).all()
 
 
