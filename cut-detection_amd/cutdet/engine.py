@@ -270,18 +270,19 @@ class Engine:
             raise RuntimeError(f"scores must be a tensor on {self.device} (got {getattr(scores, 'device', type(scores))})")
         if scores.dtype not in SCORE_TYPES:
             raise TypeError(f"scores must be float32, bfloat16 or float16, got {scores.dtype}")
-        if scores.dim() != 2 or not 1 <= scores.shape[1] <= 1 << 30:
-            raise ValueError(f"scores must be [n, k] with 1 to 2^30 classes, got {tuple(scores.shape)}")
-        return scores if scores.shape[1] == 1 or scores.stride(1) == 1 else scores.contiguous()
+        shape = scores.shape
+        if len(shape) != 2 or not 1 <= shape[1] <= 1 << 30:
+            raise ValueError(f"scores must be [n, k] with 1 to 2^30 classes, got {tuple(shape)}")
+        return scores if shape[1] == 1 or scores.stride(1) == 1 else scores.contiguous()
 
     def _per_row(self, t, name, dtype, n, *more):
         """None, or a tensor [n, *more] of `dtype` on the engine's GPU, made contiguous."""
         if t is None:
             return None
+        if torch.is_tensor(t) and t.dtype == dtype and t.shape == (n, *more) and t.device == self.device:
+            return t.contiguous()
         self._check_dev(t, name, dtype)
-        if tuple(t.shape) != (n, *more):
-            raise ValueError(f"{name} must have shape {(n, *more)}, got {tuple(t.shape)}")
-        return t.contiguous()
+        raise ValueError(f"{name} must have shape {(n, *more)}, got {tuple(t.shape)}")
 
     def _grad_rows(self, out, scores):
         """The tensor to write the scores' gradient to."""
