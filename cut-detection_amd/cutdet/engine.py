@@ -295,6 +295,13 @@ class Engine:
         return out
 
     @staticmethod
+    def _changed(out):
+        """Tells autograd that the caller's tensor has been written to: where it had been saved for a backward pass
+        (the scores themselves), that pass raises, as after an in-place operation of torch."""
+        if out is not None:
+            torch.autograd.graph.increment_version(out)
+
+    @staticmethod
     def _row_stride(t):
         return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
@@ -353,6 +360,7 @@ class Engine:
                                             self._row_stride(scores), float(temperature), _ptr(ids), _ptr(stats),
                                             _ptr(entropy), _ptr(grad_logp), _ptr(grad_entropy), _ptr(grad),
                                             self._row_stride(grad), self._stream()))
+            self._changed(out)
         return grad
 
     def _teacher(self, ids, scores, n):
@@ -390,6 +398,7 @@ class Engine:
                                  SCORE_TYPES[teacher_scores.dtype], teacher_ids.shape[1], _ptr(weights),
                                  _ptr(res["stats"]), _ptr(res["loss"]), _ptr(res.get("grad")),
                                  self._row_stride(res["grad"]) if grad else 0, _ptr(ws), size, self._stream()))
+            self._changed(out)
         return res
 
     def distill_backward(self, scores, teacher_ids, teacher_scores, stats, grad_loss, weights=None, temperature=1.0,
@@ -411,6 +420,7 @@ class Engine:
                                           _ptr(teacher_scores), SCORE_TYPES[teacher_scores.dtype],
                                           teacher_ids.shape[1], _ptr(weights), _ptr(stats), _ptr(grad_loss),
                                           _ptr(grad), self._row_stride(grad), self._stream()))
+            self._changed(out)
         return grad
 
     def rle(self, cls, maxv, frame_offset=0, cap=None):
