@@ -533,16 +533,30 @@ int check_rows(const char* name, const cd_handle* h, const RowsIn& in) {
     }
     return CD_OK;
 }
+// Whether any of n rows of `len` bytes at a, a + sa, ... has a byte in common with those at b, b + sb, ..; sb >= len.  Rows
+// of two buffers may lie between one another (the halves of a wider row).
+bool rows_overlap(int64_t a, int64_t sa, int64_t b, int64_t sb, int64_t n, int64_t len) {
+    if (a >= b + (n - 1) * sb + len || b >= a + (n - 1) * sa + len) return false;
+    // a row at p against the rows of b numbered lo..hi: only the two around p can reach it
+    auto hits = [&](int64_t p, int64_t lo, int64_t hi) {
+        const int64_t d = p - b, below = d / sb - (d % sb < 0);
+        auto reaches = [&](int64_t j) { return j >= lo && j <= hi && std::llabs(d - j * sb) < len; };
+        return reaches(below) || reaches(below + 1);
+    };
+    if (sa == sb) return hits(a, 1 - n, n - 1);           // row i of a and row j of b: as row 0 and row j - i
+    for (int64_t i = 0; i < (sa ? n : 1); ++i)
+        if (hits(a + i * sa, 0, n - 1)) return true;
+    return false;
+}
 int check_grad(const char* name, const RowsIn& in, const void* grad, int64_t stride) {
     const int size = in.type == CD_T_F32 ? 4 : 2;
     if (reinterpret_cast<uintptr_t>(grad) % size || stride < in.k || stride > ((int64_t)1 << 40) / in.n * 256) {
         set_error("%s: gradient misaligned or its row stride %lld below %d classes", name, (long long)stride, in.k);
         return CD_EINVAL;
     }
-    const char *a = static_cast<const char*>(in.x), *b = static_cast<const char*>(grad);
-    const char *a1 = a + ((in.n - 1) * in.stride + in.k) * size, *b1 = b + ((in.n - 1) * stride + in.k) * size;
-    const bool own = a == b && (in.n == 1 || in.stride == stride);
-    if (!own && a < b1 && b < a1) {
+    const bool own = in.x == grad && (in.n == 1 || in.stride == stride);
+    if (!own && rows_overlap(reinterpret_cast<intptr_t>(in.x), in.stride * size, reinterpret_cast<intptr_t>(grad),
+                             stride * size, in.n, (int64_t)in.k * size)) {
         set_error("%s: gradient overlaps with the scores", name);
         return CD_EINVAL;
     }
