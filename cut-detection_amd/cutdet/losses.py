@@ -6,7 +6,7 @@ the probabilities.  The scores may be float32, bfloat16 or float16 [n, k] on an 
 
 For a step that is captured into a HIP graph, or that needs nothing but the loss and its gradient, call
 Engine.distill(..., grad=True) (one pass for both) or Engine.log_probs and log_probs_backward: they use no autograd graph.
-These functions refuse scores that require gradients while a stream is being captured.
+These functions refuse scores that require gradients, and their backward passes, while a stream is being captured.
 """
 import torch
 
@@ -19,13 +19,17 @@ def _engine(scores):
     return api.default_engine(scores.device)
 
 
-def _not_captured(scores):
-    if torch.is_tensor(scores) and scores.is_cuda and scores.requires_grad and torch.is_grad_enabled() and \
-            torch.cuda.is_current_stream_capturing():
+def _not_captured():
+    if torch.cuda.is_current_stream_capturing():
         # autograd keeps one accumulation node per leaf, tied to the stream of its first use; where an eager graph of
         # the same leaves is alive, a captured backward would pull that stream into the capture, which can end the process
         raise RuntimeError("gradients of a leaf cannot be captured safely into a HIP graph: use Engine.distill(..., "
                            "grad=True) or Engine.log_probs_backward there")
+
+
+def _check_scores(scores):
+    if torch.is_tensor(scores) and scores.is_cuda and scores.requires_grad and torch.is_grad_enabled():
+        _not_captured()
 
 
 def _constant(t, name):
@@ -47,6 +51,7 @@ class _LogProbs(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_logp, grad_entropy):
+        _not_captured()                              # (the forward call may have been an eager one)
         scores, ids, stats, entropy = ctx.saved_tensors
         if grad_logp is None and grad_entropy is None:
             return None, None, None
@@ -66,6 +71,7 @@ class _Distill(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_loss):
+        _not_captured()
         scores, teacher_ids, teacher_scores, weights, stats = ctx.saved_tensors
         grad = ctx.engine.distill_backward(scores, teacher_ids, teacher_scores, stats, grad_loss, weights,
                                            ctx.temperature)
@@ -78,7 +84,7 @@ def log_probs(scores, ids, temperature=1.0):
     cross-entropy of the labels."""
     if not torch.is_tensor(ids):
         raise TypeError("ids must be an int64 tensor [n]")
-    _not_captured(scores)
+    _check_scores(scores)
     return _LogProbs.apply(scores, ids, float(temperature))
 
 
@@ -88,5 +94,5 @@ def distill_loss(scores, teacher_ids, teacher_scores, weights=None, temperature=
     top=...) of the teacher's scores gives them).  Differentiable with respect to the scores only."""
     _constant(teacher_scores, "teacher_scores")
     _constant(weights, "weights")
-    _not_captured(scores)
+    _check_scores(scores)
     return _Distill.apply(scores, teacher_ids, teacher_scores, weights, float(temperature))
