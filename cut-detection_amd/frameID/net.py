@@ -148,8 +148,15 @@ class Validation:
         self.net = net
         self.teacher = teacher
         self.per_frame = bool(per_frame)
-        self.rows = []                # per batch: what `per_frame` and `teacher` ask for, on the GPU
         dev = net.engine.device
+        # per batch: what `per_frame` and `teacher` ask for, on the GPU; first of no frame, so that it is there without batches
+        row, f32 = {}, torch.zeros((0,), device=dev)
+        if per_frame:
+            top = f32.reshape(0, min(2, n_classes))
+            row = {"logp": f32, "entropy": f32, "top_ids": top.long(), "top_logp": top}
+        if teacher is not None:
+            row["divergence"] = f32
+        self.rows = [row]
         self.correct = torch.zeros((n_classes,), dtype=torch.int64, device=dev)
         self.total = torch.zeros((n_classes,), dtype=torch.int64, device=dev)
         self.loss_sum = torch.zeros((1,), dtype=torch.float64, device=dev)
@@ -175,8 +182,8 @@ class Validation:
         correct, total = self.correct.cpu().tolist(), self.total.cpu().tolist()
         frames = sum(total)
         extra = {}
-        if self.rows:
-            per = {k: torch.cat([r[k] for r in self.rows]).cpu() for k in self.rows[0]}
+        per = {k: torch.cat([r[k] for r in self.rows]).cpu() for k in self.rows[0]}
+        if per:
             if "divergence" in per:
                 extra["divergence"] = float(per["divergence"].double().mean())
             extra["per_frame"] = per
