@@ -256,7 +256,9 @@ int cd_eval_accumulate(cd_handle* h, const float* logits, const int64_t* labels,
  * The calls use nothing of the handle but its device: they may overlap with other calls of the same handle, on any
  * streams.  They allocate nothing and may be captured into a HIP graph; `workspace` (cd_rows_workspace bytes of device
  * memory, 16-byte aligned; NULL where that is 0) holds values of one call only while that call's work runs.  Results do not depend on timing: two calls
- * on the same inputs give the same bits. */
+ * with the same arguments give the same bits.  The same values at another alignment may not: a row's sums are added in an
+ * order that depends on where in a 128-byte line it begins (in cd_distill with `grad`, the gradient's row), and on whether
+ * `grad` is given. */
 enum { CD_T_F32 = 0, CD_T_BF16 = 1, CD_T_F16 = 2 };      /* element types of scores and their gradients */
 
 /* Bytes of device memory that cd_log_probs (`top` alternatives) or cd_distill (top = 0) needs beside its outputs for n
@@ -266,7 +268,8 @@ size_t cd_rows_workspace(int64_t n, int n_classes, int score_type, int top);
 /* Of every row the log probability of class ids[row] (logp f32 [n]; 0 where the id is skipped), the entropy
  * -sum p ln p (entropy f32 [n]) and the `top` (0 .. 64, at most n_classes) classes with the highest scores and their
  * log probabilities (top_ids i64, top_logp f32 [n][top]; equal scores in the order of their index).  stats f32 [n][2]:
- * the row's largest score and sum exp(z - max z), for the backward call.  ids and logp may be NULL together, entropy
+ * the row's largest score and S = sum exp(z - max z), for the backward call (S is relative to max z log2(e) as rounded to 32
+ * bits: max z + ln S is ln sum exp z to 2^-24 |max z|).  ids and logp may be NULL together, entropy
  * may be NULL, top_ids and top_logp may be NULL with top = 0. */
 int cd_log_probs(cd_handle* h, const void* scores, int score_type, int64_t n, int n_classes, int64_t row_stride,
                  float temperature, const int64_t* ids, int top, float* stats, float* logp, float* entropy,
@@ -276,7 +279,8 @@ int cd_log_probs(cd_handle* h, const void* scores, int score_type, int64_t n, in
  * their type: grad [n][n_classes], grad_stride elements (>= n_classes) between rows.  stats and entropy: of the forward
  * call.  grad_logp (with ids) or grad_entropy (with entropy) may be NULL.  A row that no gradient reaches (its id skipped or
  * its grad_logp 0, and its grad_entropy 0) has gradient 0 whatever its scores.  grad may be the scores' own memory with the
- * scores' stride, and must not overlap with it otherwise. */
+ * scores' stride; otherwise no row of it may overlap with a row of scores (rows of one may lie between rows of the other), nor
+ * any with the other arguments. */
 int cd_log_probs_backward(cd_handle* h, const void* scores, int score_type, int64_t n, int n_classes,
                           int64_t row_stride, float temperature, const int64_t* ids, const float* stats,
                           const float* entropy, const float* grad_logp, const float* grad_entropy, void* grad,
@@ -288,7 +292,7 @@ int cd_log_probs_backward(cd_handle* h, const void* scores, int score_type, int6
  * 0..n_classes-1 marks an unused entry, whose score does not count; a class may be named more than once.  teacher_scores
  * [n][entries] of teacher_type: scores or log probabilities, as cd_log_probs gives them (q does not depend on a constant
  * added to a row).  weights f32 [n] or NULL (all 1): a row of weight 0 is not read, and its loss and gradient are 0, as
- * are those of a row without used entries.  loss f32 [n]; stats f32 [n][2] as in cd_log_probs.
+ * are those of a row without used entries.  loss f32 [n]; stats f32 [n][2] as in cd_log_probs (-inf and 0 for a row of weight 0).
  * grad: NULL, or [n][n_classes] of score_type for the gradient of the sum of the losses: w T (p - q), rounded once. May
  * be the scores' own memory as in cd_log_probs_backward. */
 int cd_distill(cd_handle* h, const void* scores, int score_type, int64_t n, int n_classes, int64_t row_stride,

@@ -57,3 +57,21 @@ def test_a_few_high_classes_before_many_equal_ones(eng, n, k, dtype, threads, be
     one = torch.ones((n, 1), device="cuda")
     close(eng.distill(x, ids[:, None], one)["loss"], -want, tol)
     close(eng.distill(x, ids[:, None], one, grad=True, out=x)["loss"], -want, tol)
+
+
+@pytest.mark.parametrize("k", [5, 600, 9000, 100000])
+@pytest.mark.parametrize("level", [-7e5, -3e4, 0.0, 12.0, 1e5, 7e5, 2e6])
+def test_maximum_and_sum_give_the_logarithm_of_the_sum(eng, k, level):
+    """stats: max z + ln S is ln sum exp z to the rounding of max z log2(e) to 32 bits, which S is relative to."""
+    n, t = 6, 0.8
+    g = torch.Generator().manual_seed(3)
+    x = (level + torch.randn((n, k), generator=g) * 2).float().cuda()
+    want = torch.logsumexp(x.double() / t, 1)
+    for stats in (eng.log_probs(x, temperature=t)["stats"],
+                  eng.distill(x, torch.zeros((n, 1), dtype=torch.int64, device="cuda"), torch.zeros((n, 1), device="cuda"),
+                              temperature=t)["stats"]):
+        assert torch.equal(stats[:, 0], x.amax(1))
+        z = stats[:, 0].double() / t
+        d = (z + stats[:, 1].double().log() - want).abs()
+        # besides: c = log2(e) / T of the scores' distances from the maximum, at most 16, is off by 2 u
+        assert (d <= ref.U * (1 + 1e-5) * z.abs() + ref.row_error(k) + 32 * ref.U).all(), d.max()
