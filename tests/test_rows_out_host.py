@@ -26,6 +26,7 @@ def host_engine(monkeypatch):
     eng._stream = lambda: None
     eng.library = Library()
     monkeypatch.setattr(engine, "lib", eng.library)
+    monkeypatch.setattr(engine, "_rows_workspace", lambda *args: 0)
     return eng
 
 
