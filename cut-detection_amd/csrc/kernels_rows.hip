@@ -298,7 +298,10 @@ __device__ __forceinline__ void write_top(const LogProbsArgs& A, int64_t row, in
 // piece that has their maximum), collect those that reach T in a list, and the list is ranked by counting.  Scores equal
 // to T may be very many (a mask): where a wave finds more than kDense threads at T it leaves them, and the
 // lowest-numbered classes at T are found by a scan in the order of the classes, which then ends early.  A list that
-// overflows all the same (scores laid out against the threads), and NaN, take one scan per class.
+// overflows all the same, and NaN, take one scan per alternative, which is slow.  A list overflows where T is a mask's value
+// and most threads of one wave have an allowed score besides their masked ones: that wave collects all of its masked scores.
+// Then at least 40 groups have an allowed score, and fewer than there are alternatives: a short run of allowed classes and
+// more than 40 alternatives (4096 x 128000 bf16, all but 400 consecutive classes at -inf: 189 us with 20 alternatives, 33 ms with 64).
 constexpr int kDense = 24, kFewTops = 24;
 template <int THREADS> struct BlockShared {
     static constexpr int kWaves = THREADS / 64, kList = 1024;
@@ -1257,10 +1260,11 @@ __global__ __launch_bounds__(256) void distill_group_kernel(DistillArgs A) {
 
 // ================================================================================== one wave per row, up to 4096 scores
 // The row stays in the wave's registers, no barrier, and four rows to a workgroup: 30000 x 2000 bf16 with 20 alternatives
-// takes 61 us so and 152 us with a workgroup per row, 30000 x 4000 loss and gradient 100 us and 183 us.  Beyond 2048
-// scores (log_probs: its alternatives) or 8 KB the registers leave too few waves.  Up to 512 scores one score at a time, score i in lane
+// takes 57 us so and 152 us with a workgroup per row, 30000 x 4000 loss and gradient 92 us and 183 us.  Beyond 2048
+// scores for log_probs, whose alternatives need registers of their own (it goes by the length alone, so without alternatives too),
+// and beyond 8 KB for the others the registers leave too few waves.  Up to 512 scores one score at a time, score i in lane
 // i % 64; above that vectors of 16 bytes, so that every lane has some, and the rest of a row one score per lane (50000 x
-// 1000 bf16: 32 us with vectors, 83 us without).
+// 1000 bf16: 27 us with vectors, 83 us without).
 constexpr int kWaveClasses = 2048, kWaveBytes = 8192;
 
 template <int TYPE, int N> struct SpreadRow {
@@ -1496,7 +1500,8 @@ int elem_size(int type) { return type == CD_T_F32 ? 4 : 2; }
 // with 512; 20000 x 16000 bf16 174, 159, 209; 8000 x 64000 bf16 327, 243, 215; 4096 x 128000 bf16 263 with 256, 217 with 512, 249
 // with 1024).  With few rows a row's own time counts (200 x 32000 bf16: 20 us with 128, 12.9 with 256, 10 with 512; 64 x
 // 131072 bf16: 29 with 256, 19 with 512, 16 with 1024).  Where 256 threads, six workgroups to a CU, hold all rows at
-// once and 512, three, would need a second round: 256 (1000 x 50021 f32: 39 us against 44).
+// once and 512, three, would need a second round: 256 (1000 x 50021 f32: 39 us against 44; the band of 769 to 1536 rows
+// follows from the numbers of workgroups that 256 CUs hold, and is measured at this size alone).
 int block_threads(const RowsIn& in) {
     const int64_t bytes = (int64_t)in.k * elem_size(in.type);
     if (bytes <= 16384) return in.n >= 512 ? 128 : 256;
@@ -1528,7 +1533,7 @@ int block_threads(const RowsIn& in) {
         else { CD_BY_TYPE((in).type, CD_VECTORS, 2, CALL); }                                       \
     } while (0)
 #define CD_VECTORS(TY, KILO, CALL) CALL(TY, VectorRow<TY, 16 / Elem<TY>::kVec * KILO>)
-// ... and of the 16-bit scores beyond that a wave takes where there are no alternatives to find
+// ... and of 16-bit scores beyond that, up to kWaveBytes: for gradients and for distill's loss, not for log_probs
 #define CD_WAVE_ROWS_16(in, CALL)                                                                  \
     do {                                                                                           \
         if ((in).type == CD_T_BF16) { CALL(CD_T_BF16, VectorRow<CD_T_BF16, 8>); }                  \
@@ -1545,7 +1550,8 @@ constexpr int64_t kSplitBytes = 128 << 10, kSplitRows = 64;
 
 // Workgroups per row of the calls that need a second kernel to join them: few rows, long enough that the second launch costs
 // less than one CU's reading (1 x 262144 f32, loss alone: 7.5 us split, 41 us with one workgroup; 16 x 131072 bf16 with 20
-// alternatives 12.3 and 14.7; 64 x 131072 bf16 15.2 and 15.7).
+// alternatives 12.3 and 14.7; 64 x 131072 bf16 15.2 and 15.7).  The limit is right for rows of that length; longer ones lose by it:
+// 65 x 262144 f32 takes 24 us with a workgroup per row, 64 rows 18 us split.
 static int join_parts(int64_t n, int k, int type) {
     const int64_t bytes = (int64_t)k * elem_size(type);
     if (bytes < kSplitBytes || n > kSplitRows) return 1;

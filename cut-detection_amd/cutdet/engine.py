@@ -344,7 +344,7 @@ class Engine:
                            out=None):
         """Gradient of sum(grad_logp * logp + grad_entropy * entropy) with respect to the scores, in their type.
         `stats` and `entropy` are those of log_probs on the same scores; `ids` is needed with `grad_logp` and `entropy`
-        with `grad_entropy`.  `out` may be the scores themselves."""
+        with `grad_entropy`.  `out` may be the scores themselves, which autograd then takes for changed in place."""
         scores_in, scores = scores, self._score_rows(scores)
         n, k = scores.shape
         ids = self._per_row(ids, "ids", torch.int64, n)
